@@ -313,6 +313,111 @@ int tsw_place_segments_static(int device, const tsw_segment* segs, int n, uint32
  * caller's current device is unchanged by both calls.  No counterpart in the reference. */
 int tsw_place_segments_static_status(int device, void* stream, uint32_t* status, int clear);
 
+/* Key/value cache operators: what a served language-model function needs beside its weights in the
+ * same memory.  No counterpart in the reference, which forwards the client's own kernels.
+ *
+ * Keys and values live in pages of page_size tokens anywhere in one address range (a block of the
+ * pool, a function's parameter, any device allocation).  Own tokens of sequence b are numbered from
+ * 0; token j lies in page page_table[b * table_stride + j / page_size] at place j % page_size.  A
+ * prefix that all sequences share -- a function's own prompt -- is one more list of pages, in the
+ * same range or in another one (the function's parameters, say, which a swap-in brings along with
+ * its weights).
+ *
+ * A call handles `tokens` rows of new tokens.  Rows cu_q[b] .. cu_q[b+1] - 1 belong to sequence b and
+ * are its LAST tokens: with n rows and seq_lens[b] own tokens (the new ones included), row i of the
+ * sequence is own token seq_lens[b] - n + i.  Rows outside cu_q[0] .. cu_q[batch] belong to nobody
+ * and everything that corresponds to them is left as it was.  All three tables are int32 in
+ * device memory and are read on the device, so a captured call follows their contents on replay.
+ *
+ * Types: TSW_F16 and TSW_BF16, the same for all operands of a call; sums, statistics and
+ * rotations are held in 32 bits or more, and each result is rounded once.  Strides are in bytes;
+ * the elements of a head are contiguous.  Head h of the queries reads key head
+ * h / (q_heads / kv_heads).
+ *
+ * The calls take a device ordinal and a cudaStream_t of that device, allocate nothing, wait for nothing
+ * on the host, leave the caller's current device as it was, and may be captured into a graph.  Bad
+ * arguments that the host can see are refused with TSW_ERR_INVALID before anything is launched.  What
+ * only the device sees -- a page number outside the cache, a length beyond the table, rows out of
+ * order -- is never followed out of bounds: it is recorded in a word per device that
+ * tsw_kv_status reads, and what was computed for that sequence is unspecified.  A page that
+ * takes new tokens belongs to one sequence: if two sequences name it, either's tokens may stay. */
+enum { TSW_F16 = 0, TSW_BF16 = 1 };
+typedef struct {
+    uint64_t k, v;          /* page 0, token 0, head 0 of the keys and of the values */
+    uint64_t k_page_stride, k_token_stride, k_head_stride;
+    uint64_t v_page_stride, v_token_stride, v_head_stride;
+    uint32_t pages;         /* pages in the range: valid numbers are 0 .. pages - 1 */
+    uint32_t page_size;     /* tokens to a page */
+} tsw_kv_pages;
+typedef struct {
+    uint64_t page_table;    /* int32 [batch][table_stride]; may be null when no sequence has own tokens */
+    uint64_t seq_lens;      /* int32 [batch] */
+    uint64_t cu_q;          /* int32 [batch + 1], not decreasing */
+    uint32_t batch;
+    uint32_t table_width;   /* valid entries of a table row: own tokens end at table_width * page_size */
+    uint32_t table_stride;  /* entries from one row to the next */
+    uint32_t tokens;        /* rows of the query, key, value and output operands */
+} tsw_kv_batch;
+
+/* Append the new tokens' keys and values to the cache.  Keys (and queries, when q is given) are first
+ * rotated by position: with p = position_offset + own token number and angle a_c = p * inv_freq[c]
+ * (double, formed and reduced in 64 bits), each pair (x, y) becomes (x cos a - y sin a,
+ * x sin a + y cos a); pair c is elements (c, c + rotary_dim / 2), or (2c, 2c + 1) with
+ * interleaved != 0.  Elements from rotary_dim on are copied.  rotary_dim = 0 rotates nothing.  q_out
+ * may be q itself.  Rows whose own token number is negative (more new rows than seq_lens) are skipped. */
+typedef struct {
+    tsw_kv_pages cache;
+    tsw_kv_batch batch;
+    uint64_t q, q_out, k, v;             /* [tokens][heads][head_dim]; q = q_out = 0: keys and values only */
+    uint64_t q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride;
+    uint64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    uint64_t inv_freq;                   /* double [rotary_dim / 2] in device memory */
+    uint64_t position_offset;            /* tokens before own token 0 (the shared prefix's length), below 2^32 */
+    uint32_t dtype, q_heads, kv_heads, head_dim, rotary_dim, interleaved;
+} tsw_kv_append_args;
+int tsw_kv_append(int device, const tsw_kv_append_args* args, void* stream);
+
+/* Attention of the new tokens over the shared prefix and their sequence's own pages:
+ * out = softmax(scale * q k^T) v.  A row sees the whole prefix and, with causal != 0, the own tokens
+ * up to its own number; with causal = 0 all own tokens of its sequence (an encoder's states, say).
+ * A row that sees nothing gets zeros and a log-sum of -inf.  The prefix is read once for all
+ * sequences, not once for each.  What lies in a page behind the last token is not read into any
+ * result, whatever its bits.  A value that is infinite or NaN reaches every row of its own sequence in
+ * the same call (for a prefix value: every row), also the rows that stand before it.
+ * lse, when given, receives ln(sum of exp) per row and head, float [tokens][q_heads].
+ * The result is the same bit for bit on every call with the same arguments and tables.
+ * workspace: tsw_prefix_attention_workspace(args) bytes of device memory, 256-byte aligned, in use until the
+ * call has finished on the stream: calls that may overlap need one each.  Its contents do not matter. */
+typedef struct {
+    tsw_kv_pages cache;
+    tsw_kv_pages prefix;                 /* where the prefix pages lie; often equal to cache */
+    tsw_kv_batch batch;
+    uint64_t prefix_table;               /* int32 [ceil(prefix_len / prefix.page_size)] in device memory */
+    uint64_t q, out;                     /* [tokens][q_heads][head_dim] */
+    uint64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+    uint64_t lse;                        /* optional (0) */
+    uint64_t workspace, workspace_bytes;
+    uint32_t prefix_len;
+    uint32_t max_q;                      /* no sequence has more new rows than this */
+    uint32_t dtype, q_heads, kv_heads, head_dim, causal;
+    float scale;
+} tsw_prefix_attention_args;
+int tsw_prefix_attention_workspace(const tsw_prefix_attention_args* args, uint64_t* bytes);
+int tsw_prefix_attention(int device, const tsw_prefix_attention_args* args, void* stream);
+
+/* What the two operators' kernels found wrong in device tables since the word was last cleared: a sum
+ * of TSW_KV_*; 0 = nothing.  Synchronises `stream`; clear != 0 resets the word. */
+enum { TSW_KV_BAD_PAGE = 1, TSW_KV_BAD_LENGTH = 2, TSW_KV_BAD_ROWS = 4, TSW_KV_WAIT_GAVE_UP = 8 };
+int tsw_kv_status(int device, void* stream, uint32_t* status, int clear);
+
+/* The same operators on a function's own memory: every address in `args` except workspace is a client address of
+ * `func` and is translated as the executor translates a kernel's arguments (cuda_server.hpp:1265-1268);
+ * each operand must lie inside one block of the function (TSW_ERR_NOT_FOUND otherwise).  Parameters
+ * that are still being swapped in are waited for on the stream, as in tsw_translate_async, and are recorded as
+ * accessed. */
+int tsw_func_kv_append(tsw_engine* e, const char* func, const tsw_kv_append_args* args, void* stream);
+int tsw_func_prefix_attention(tsw_engine* e, const char* func, const tsw_prefix_attention_args* args, void* stream);
+
 /* Counters: kernels launched by this engine, bytes they were asked to move, and device
  * time of the last swap on the transfer stream (CUDA events), in nanoseconds. */
 int tsw_stats(tsw_engine* e, uint64_t* kernel_launches, uint64_t* bytes_moved, uint64_t* last_swap_device_ns);

@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libtorpor_swap.so")
 OK = 0
 ERR_INVALID, ERR_NO_DEVICE, ERR_CUDA, ERR_POOL_EXHAUSTED, ERR_UNKNOWN_MODEL = -1, -2, -3, -4, -5
 ERR_TIMEOUT, ERR_NOT_FOUND, ERR_BUFFER, ERR_STATE, ERR_KERNEL = -6, -7, -8, -9, -10
+F16, BF16 = 0, 1
 READY_HOST, READY_PINNED, READY_CUDA = 0, 1, 2
 MODEL_FULL, MODEL_INCOMPLETE, MODEL_PARTIAL, MODEL_NODATA = 0, 1, 2, 3
 POOL_BUDDY, POOL_FIXED = 0, 1
@@ -67,6 +68,39 @@ class Publish(C.Structure):
 
 class IpcRegion(C.Structure):
     _fields_ = [("base", C.c_uint64), ("size", C.c_uint64), ("handle", C.c_ubyte * 64)]
+
+
+class KvPages(C.Structure):
+    _fields_ = [("k", C.c_uint64), ("v", C.c_uint64),
+                ("k_page_stride", C.c_uint64), ("k_token_stride", C.c_uint64), ("k_head_stride", C.c_uint64),
+                ("v_page_stride", C.c_uint64), ("v_token_stride", C.c_uint64), ("v_head_stride", C.c_uint64),
+                ("pages", C.c_uint32), ("page_size", C.c_uint32)]
+
+
+class KvBatch(C.Structure):
+    _fields_ = [("page_table", C.c_uint64), ("seq_lens", C.c_uint64), ("cu_q", C.c_uint64), ("batch", C.c_uint32),
+                ("table_width", C.c_uint32), ("table_stride", C.c_uint32), ("tokens", C.c_uint32)]
+
+
+class KvAppendArgs(C.Structure):
+    _fields_ = [("cache", KvPages), ("batch", KvBatch),
+                ("q", C.c_uint64), ("q_out", C.c_uint64), ("k", C.c_uint64), ("v", C.c_uint64),
+                ("q_token_stride", C.c_uint64), ("q_head_stride", C.c_uint64),
+                ("q_out_token_stride", C.c_uint64), ("q_out_head_stride", C.c_uint64),
+                ("k_token_stride", C.c_uint64), ("k_head_stride", C.c_uint64),
+                ("v_token_stride", C.c_uint64), ("v_head_stride", C.c_uint64),
+                ("inv_freq", C.c_uint64), ("position_offset", C.c_uint64),
+                ("dtype", C.c_uint32), ("q_heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("rotary_dim", C.c_uint32), ("interleaved", C.c_uint32)]
+
+
+class PrefixAttentionArgs(C.Structure):
+    _fields_ = [("cache", KvPages), ("prefix", KvPages), ("batch", KvBatch), ("prefix_table", C.c_uint64),
+                ("q", C.c_uint64), ("out", C.c_uint64), ("q_token_stride", C.c_uint64), ("q_head_stride", C.c_uint64),
+                ("out_token_stride", C.c_uint64), ("out_head_stride", C.c_uint64), ("lse", C.c_uint64),
+                ("workspace", C.c_uint64), ("workspace_bytes", C.c_uint64), ("prefix_len", C.c_uint32), ("max_q", C.c_uint32),
+                ("dtype", C.c_uint32), ("q_heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("causal", C.c_uint32), ("scale", C.c_float)]
 
 
 # Every symbol include/torpor_swap.h declares: name -> (restype, argtypes)
@@ -126,6 +160,12 @@ SIGNATURES = {
     "tsw_place_segments_pipelined": (_i32, [_vp, _vp, _i32, C.c_uint32, C.c_uint32, C.c_uint32, _vp, C.c_uint32, _i32]),
     "tsw_place_segments_static": (_i32, [_i32, _vp, _i32, C.c_uint32, C.c_uint32, C.c_uint32, _vp, _vp]),
     "tsw_place_segments_static_status": (_i32, [_i32, _vp, C.POINTER(C.c_uint32), _i32]),
+    "tsw_kv_append": (_i32, [_i32, C.POINTER(KvAppendArgs), _vp]),
+    "tsw_prefix_attention_workspace": (_i32, [C.POINTER(PrefixAttentionArgs), _pu64]),
+    "tsw_prefix_attention": (_i32, [_i32, C.POINTER(PrefixAttentionArgs), _vp]),
+    "tsw_kv_status": (_i32, [_i32, _vp, C.POINTER(C.c_uint32), _i32]),
+    "tsw_func_kv_append": (_i32, [_vp, _cp, C.POINTER(KvAppendArgs), _vp]),
+    "tsw_func_prefix_attention": (_i32, [_vp, _cp, C.POINTER(PrefixAttentionArgs), _vp]),
     "tsw_stats": (_i32, [_vp, _pu64, _pu64, _pu64]),
     "tsw_evictor_create": (_i32, [_cp, _i32, _u64, C.POINTER(_vp)]),
     "tsw_evictor_destroy": (_i32, [_vp]),
