@@ -1,0 +1,221 @@
+// The dealing of the attention kernel's work (csrc/kv_dealing.hpp), run on the host for random batches: every
+// (row tile, head, key tile) is taken exactly once; the warps that walk the tiles and the rows' warps see
+// the same order; what the joining kernel reads of a row is exactly what was written for it; every index
+// stays inside its table or the workspace.
+//   kv_dealing_probe SEED CASES
+#include <cstdio>
+#include <cstdlib>
+#include <map>
+#include <random>
+#include <set>
+#include <tuple>
+#include <vector>
+
+#include "../torpor_b200/csrc/kv_dealing.hpp"
+
+using namespace tsw;
+
+#define REQUIRE(x)                                                              \
+    do {                                                                        \
+        if (!(x)) {                                                             \
+            printf("case %d line %d: %s\n", g_case, __LINE__, #x);              \
+            exit(1);                                                            \
+        }                                                                       \
+    } while (0)
+static int g_case;
+
+int main(int argc, char** argv) {
+    std::mt19937 rng(argc > 1 ? atoi(argv[1]) : 1);
+    const int cases = argc > 2 ? atoi(argv[2]) : 100;
+    auto pick = [&](int lo, int hi) { return (int)(lo + rng() % (uint32_t)(hi - lo + 1)); };
+    long long tiles_seen = 0, parts_seen = 0;
+    for (g_case = 0; g_case < cases; ++g_case) {
+        // ---- a batch, sometimes with wild tables
+        const int batch = pick(0, 3) ? pick(1, 12) : pick(1, 500), wild = pick(0, 9) == 0;
+        const int page_size = 1 << pick(0, 8), kv_heads = pick(1, 6), groups[] = {1, 2, 3, 4, 7, 8, 16, 128}, group = groups[pick(0, 7)];
+        const int q_most = pick(0, 2) == 0 ? 1 : pick(0, 1) ? pick(1, 8) : pick(1, 400);
+        const int own_most = pick(0, 3) == 0 ? pick(0, 40) : pick(0, 3000), sms = pick(0, 2) ? 148 : pick(1, 20);
+        std::vector<int> cu(batch + 1), lens(batch);
+        int at = pick(0, 3) ? 0 : pick(0, 5), widest = 0;
+        for (int b = 0; b < batch; ++b) {
+            cu[b] = at;
+            at += pick(0, 4) ? pick(0, q_most) : 0;
+            lens[b] = pick(0, 5) ? pick(0, own_most) : 0;
+            widest = std::max(widest, lens[b]);
+        }
+        cu[batch] = at;
+        const int tokens = at + pick(0, 4), width = (widest + page_size - 1) / page_size + pick(0, 2);
+        if (tokens == 0) continue;
+        if (wild)
+            for (int i = 0; i < 3; ++i) {
+                const int odd[] = {-5, 1 << 30, 0x7fffffff, (int)0x80000000, 7};
+                (pick(0, 1) ? cu[pick(0, batch)] : lens[pick(0, batch - 1)]) = odd[pick(0, 4)];
+            }
+        tsw_prefix_attention_args a = {};
+        a.batch.seq_lens = (uint64_t)lens.data();
+        a.batch.cu_q = (uint64_t)cu.data();
+        a.batch.page_table = width ? 4096 : 0;
+        a.batch.batch = batch;
+        a.batch.table_width = a.batch.table_stride = width;
+        a.batch.tokens = tokens;
+        a.head_dim = 64;
+        a.kv_heads = kv_heads;
+        a.q_heads = kv_heads * group;
+        a.cache = tsw_kv_pages{1 << 20, 1 << 21, 4096, 4096, 4096, 4096, 4096, 4096, 100, (uint32_t)page_size};
+        a.prefix = a.cache;
+        a.prefix_len = pick(0, 2) ? pick(0, 2000) : 0;
+        a.q = a.out = 1 << 22;
+        a.q_token_stride = a.q_head_stride = a.out_token_stride = a.out_head_stride = 4096;
+        a.max_q = pick(0, 9) ? q_most : pick(0, tokens);
+        a.causal = pick(0, 1);
+        a.scale = 1.f;
+        AttentionLayout w;
+        REQUIRE(attention_layout(a, sms, &w));
+        const Deal d{a.batch, a.max_q, a.cache.page_size, a.kv_heads, a.prefix_len, a.causal, w};
+        REQUIRE(w.group * w.tile_tokens <= 128 && w.tile_tokens >= 1 && w.own_box_tokens >= 1 && w.own_box_tokens <= w.tile_tokens);
+
+        // ---- what the first CTA leaves for the joining kernel
+        std::vector<uint32_t> base(batch + 1);
+        uint32_t total = 0;
+        for (int b = 0; b < batch; ++b) {
+            SeqRows r;
+            read_rows(a.batch, b, a.max_q, page_size, r);
+            REQUIRE(r.first >= 0 && r.n >= 0 && r.first + r.n <= tokens && r.len >= 0 && r.len <= (long long)width * page_size && r.n <= (int)a.max_q);
+            base[b] = total;
+            total += sequence_tiles(d, r);
+        }
+        base[batch] = total;
+        int tok0, tok1;
+        const uint32_t rts = prefix_rows(d, tok0, tok1);
+        const uint32_t prefix_total = a.kv_heads * rts * w.prefix_tiles;
+
+        std::set<std::tuple<int, int, int, int>> done;                  // list, first token of a row tile, head, key tile
+        std::set<uint64_t> home, part;                                  // partial results written, in rows of the workspace
+        std::map<uint64_t, int> direct;
+        const uint64_t home_rows = 2ull * tokens * a.q_heads, part_rows = 4ull * w.ctas * w.part_rows;
+        for (int cta = 0; cta < (int)w.ctas; ++cta) {
+            Prologue pro = {};
+            for (int s = 0; s < 2; ++s) pro.prefix[s] = range_at(d, w.prefix_pair, prefix_total, cta, s);
+            pro.prefix_rt = std::max(1u, rts);
+            pro.tok0 = tok0;
+            pro.tok1 = tok1;
+            for (int s = 0; s < 2; ++s) {
+                const Range g = range_at(d, w.own_pair, total, cta, s);
+                const uint32_t x = g.x, left = g.end - g.x;
+                // the kernel's threads look through pieces of the sequences; one of them holds x
+                const int each = (batch + 383) / 384;
+                int found = 0;
+                for (int lo = 0; left && lo < batch; lo += each) {
+                    const int hi = std::min(batch, lo + each);
+                    if (x < base[lo] || x >= base[hi]) continue;
+                    REQUIRE(find_start(d, lo, hi, x - base[lo], left, pro.own[s]));
+                    ++found;
+                }
+                REQUIRE(found == (left ? 1 : 0));
+            }
+            // units in the walkers' order, by stream
+            std::vector<std::tuple<int, int, int, int, int>> by_stream[2], by_rows[2];    // list, b, tok, head, tile
+            Walk walk(d, pro);
+            Job j;
+            int tile;
+            bool use[2];
+            while (walk.next(d, pro, j, tile, use[0], use[1])) {
+                ++tiles_seen;
+                REQUIRE(use[0] || use[1]);
+                REQUIRE(tile >= j.kt0 && tile < j.kt1 && tile * kTile < j.keys);
+                const tsw_kv_pages& pg = j.own ? a.cache : a.prefix;
+                const int n = std::min(kTile, j.keys - tile * kTile), box = std::min((int)pg.page_size, kTile), first = tile * kTile / (int)pg.page_size;
+                const int last = first + (n + box - 1) / box - 1;
+                REQUIRE(last < (j.own ? width : ((int)a.prefix_len + page_size - 1) / page_size));
+                for (int s = 0; s < 2; ++s)
+                    if (use[s]) {
+                        const int tok = j.tok + (walk.pair && s ? (int)w.tile_tokens : 0);
+                        by_stream[s].push_back({j.own, j.b, tok, j.head, tile});
+                        REQUIRE(done.insert({j.own, tok, j.head, tile}).second);
+                    }
+            }
+            for (int s = 0; s < 2; ++s)
+                for (int own = 0; own < 2; ++own) {
+                    const bool pair = own ? w.own_pair : w.prefix_pair;
+                    Cursor cur(pro, pair ? 0 : s);
+                    while (cur.next(d, pro, own, j)) {
+                        const int seen = seen_by(j, pair, s), end = std::min(j.kt1, seen), tokens_here = pair && s ? j.n_b : j.n_a;
+                        const int tok = j.tok + (pair && s ? (int)w.tile_tokens : 0);
+                        for (int t = j.kt0; t < end; ++t) by_rows[s].push_back({own, j.b, tok, j.head, t});
+                        if (j.kt0 >= end) continue;
+                        REQUIRE(tokens_here >= 1 && tokens_here <= (int)w.tile_tokens && tok >= 0 && tok + tokens_here <= tokens);
+                        for (int i = 0; i < tokens_here * group; ++i) {
+                            const uint64_t row = (uint64_t)(tok + i / group) * a.q_heads + j.head * group + i % group;
+                            if (a.prefix_len == 0 && j.kt0 == 0 && end == seen) ++direct[row];
+                            else if (j.kt0 == 0) {
+                                const uint64_t h = home_index(d, own, row, a.q_heads);
+                                REQUIRE(h < home_rows && home.insert(h).second);
+                            } else {
+                                const uint64_t p = part_index(d, own, part_place(pair, range_index(d, pair, cta, s), s), i);
+                                REQUIRE(p < part_rows && part.insert(p).second);
+                            }
+                        }
+                    }
+                }
+            for (int s = 0; s < 2; ++s) REQUIRE(by_stream[s] == by_rows[s]);
+        }
+        // ---- the joining kernel's view: every row of a sequence
+        size_t homes_read = 0, expected = 0;
+        std::set<uint64_t> parts_read;
+        for (int b = 0; b < batch; ++b) {
+            SeqRows r;
+            read_rows(a.batch, b, a.max_q, page_size, r);
+            for (int i = 0; i < r.n; ++i)
+                for (int head = 0; head < (int)a.q_heads; ++head) {
+                    const int tok = r.first + i, kv = head / group;
+                    const uint64_t row = (uint64_t)tok * a.q_heads + head;
+                    uint32_t before = 0;
+                    for (int rt = 0; rt < i / own_item_tokens(d); ++rt) {
+                        const Cut c = cut_own(d, r, rt);
+                        before += std::max(c.kt_a, c.kt_b);
+                    }
+                    const Parts parts[2] = {prefix_parts(d, tok, kv, prefix_total), own_parts(d, r, tok, kv, base[b], before, total)};
+                    const int keys = a.causal ? std::max(0, std::min(r.len, r.len - r.n + i + 1)) : r.len;
+                    REQUIRE(wild || parts[0].has == (a.prefix_len > 0));
+                    REQUIRE(parts[1].has || keys == 0);
+                    if (!wild) {
+                        // all of a row's key tiles were taken
+                        for (int t = 0; t * kTile < keys; ++t) REQUIRE(done.count({1, tok - (i % (int)w.tile_tokens), kv, t}));
+                        for (int t = 0; t < (int)w.prefix_tiles; ++t) REQUIRE(done.count({0, tok - (tok - tok0) % (int)w.tile_tokens, kv, t}));
+                    }
+                    if (!a.prefix_len && parts[1].has && parts[1].first == parts[1].last) {
+                        REQUIRE(wild || direct[row] == 1);
+                        continue;
+                    }
+                    REQUIRE(wild || direct.count(row) == 0);
+                    for (int l = 0; l < 2; ++l) {
+                        const Parts& q = parts[l];
+                        if (!q.has) continue;
+                        const uint64_t h = home_index(d, l, row, a.q_heads);
+                        REQUIRE(wild || home.count(h));
+                        ++homes_read;
+                        const bool pair = l ? w.own_pair : w.prefix_pair;
+                        for (uint32_t k = q.first + 1; k <= q.last; ++k) {
+                            const uint64_t p = part_index(d, l, part_place(pair, k, q.half), q.place * group + head % group);
+                            REQUIRE(p < part_rows);
+                            REQUIRE(wild || part.count(p));
+                            REQUIRE(parts_read.insert(p).second || wild);
+                            ++parts_seen;
+                        }
+                    }
+                }
+        }
+        (void)expected;
+        if (!wild && cu[0] == tok0 && tok1 == cu[batch]) {
+            // nothing was written that nobody reads, except for rows of sequences longer than max_q
+            bool all = true;
+            for (int b = 0; b < batch; ++b) all = all && cu[b + 1] - cu[b] <= (int)a.max_q;
+            if (all) {
+                REQUIRE(homes_read == home.size());
+                REQUIRE(parts_read.size() == part.size());
+            }
+        }
+    }
+    printf("ok %d cases, %lld tiles, %lld continued rows\n", cases, tiles_seen, parts_seen);
+    return 0;
+}

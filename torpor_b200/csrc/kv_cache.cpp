@@ -2,7 +2,11 @@
 // function's client addresses.  The kernels are in kv_kernels.cu.
 
 #include "engine_internal.hpp"
+
+#include <atomic>
+
 #include "kv_kernels.hpp"
+#include "kv_dealing.hpp"
 
 using namespace tsw;
 
@@ -10,6 +14,7 @@ namespace {
 
 constexpr int kMaxDevices = 64;
 constexpr uint32_t kMaxHeadDim = 512;
+constexpr int kMaxSms = 160;    // what a workspace is sized for before the device is known
 
 struct DeviceGuard {            // the caller's current device is put back
     int old = -1;
@@ -25,6 +30,18 @@ int sm_count(int device, int* sms) {
         known[device].store(n, std::memory_order_relaxed);
     }
     *sms = n;
+    return TSW_OK;
+}
+
+// Address of the device's status word; the device is current.
+int status_word(int device, uint32_t** word) {
+    static std::atomic<uint32_t*> known[kMaxDevices];
+    uint32_t* w = known[device].load(std::memory_order_relaxed);
+    if (!w) {
+        TSW_CUDA(kv_status_symbol(&w));
+        known[device].store(w, std::memory_order_relaxed);
+    }
+    *word = w;
     return TSW_OK;
 }
 
@@ -215,7 +232,8 @@ int tsw_prefix_attention_workspace(const tsw_prefix_attention_args* args, uint64
     return guarded([&]() -> int {
         if (!args || !bytes) return bad("null argument");
         CHECK(check_attention(*args));
-        *bytes = 0;
+        AttentionLayout w;
+        *bytes = attention_layout(*args, kMaxSms, &w) ? w.bytes : 0;
         return TSW_OK;
     });
 }
@@ -229,7 +247,16 @@ int tsw_prefix_attention(int device, const tsw_prefix_attention_args* args, void
         DeviceGuard restore;
         int sms;
         CHECK(use_device(device, &sms));
-        TSW_CUDA(launch_prefix_attention_rows(*args, (cudaStream_t)stream));
+        AttentionLayout w;
+        if (!attention_layout(*args, std::min(sms, kMaxSms), &w)) {
+            TSW_CUDA(launch_prefix_attention_rows(*args, (cudaStream_t)stream));
+            return TSW_OK;
+        }
+        if (!args->workspace || (args->workspace & 255)) return bad("workspace must be a 256-byte aligned device address");
+        if (args->workspace_bytes < w.bytes) return fail(TSW_ERR_BUFFER, "workspace is smaller than tsw_prefix_attention_workspace asks for");
+        uint32_t* word;
+        CHECK(status_word(device, &word));
+        TSW_CUDA(launch_prefix_attention_tiles(*args, w, word, (cudaStream_t)stream));
         return TSW_OK;
     });
 }
@@ -242,7 +269,7 @@ int tsw_kv_status(int device, void* stream, uint32_t* status, int clear) {
         int sms;
         CHECK(use_device(device, &sms));
         uint32_t* word = nullptr;
-        TSW_CUDA(kv_status_symbol(&word));
+        CHECK(status_word(device, &word));
         cudaStream_t s = (cudaStream_t)stream;
         uint32_t seen = 0;
         TSW_CUDA(cudaMemcpyAsync(&seen, word, sizeof(seen), cudaMemcpyDeviceToHost, s));

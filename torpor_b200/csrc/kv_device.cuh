@@ -9,7 +9,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include "../../include/torpor_swap.h"
+#include "kv_dealing.hpp"
 
 namespace tsw {
 
@@ -49,24 +49,6 @@ __device__ __forceinline__ int find_sequence(const int* cu_q, uint32_t batch, ui
     const int b = (int)lo - 1;
     if (b < 0 || b >= (int)batch) return -1;
     return b;
-}
-
-// Rows and length of one sequence, made safe: whatever the tables hold, 0 <= first, first + n <= tokens,
-// n <= max_q and 0 <= len <= what the page table covers.  What had to be changed is recorded.
-struct SeqRows { int first, n, len; };
-__device__ __forceinline__ void read_rows(const tsw_kv_batch& t, int b, uint32_t max_q, uint32_t page_size, uint32_t* status, SeqRows& r) {
-    const int* cu = (const int*)t.cu_q;
-    const int lo = cu[b], hi = cu[b + 1];
-    int len = ((const int*)t.seq_lens)[b];
-    uint32_t bad = 0;
-    r.first = lo;
-    r.n = hi - lo;
-    if (lo < 0 || hi < lo || hi > (int)t.tokens || (uint32_t)(hi - lo) > max_q) { bad |= TSW_KV_BAD_ROWS; r.first = 0; r.n = 0; }
-    const uint64_t room = t.page_table ? (uint64_t)t.table_width * page_size : 0;
-    if (len < 0) { bad |= TSW_KV_BAD_LENGTH; len = 0; }
-    if ((uint64_t)len > room) { bad |= TSW_KV_BAD_LENGTH; len = (int)room; }
-    r.len = len;
-    if (bad) atomicOr(status, bad);
 }
 
 }  // namespace tsw

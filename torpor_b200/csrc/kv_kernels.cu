@@ -126,7 +126,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
             int j = -1, page = -1, at = 0;
             if (b >= 0) {
                 SeqRows r;
-                read_rows(a.batch, b, a.batch.tokens, a.cache.page_size, &g_kv_status, r);
+                const uint32_t wrong = read_rows(a.batch, b, a.batch.tokens, a.cache.page_size, r);
+                if (wrong) atomicOr(&g_kv_status, wrong);
                 j = (int)tok < r.first + r.n ? r.len - r.n + ((int)tok - r.first) : -1;
                 if (j >= 0) {
                     page = ((const int*)a.batch.page_table)[(uint64_t)b * a.batch.table_stride + j / (int)a.cache.page_size];
@@ -180,7 +181,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) attention_rows_kernel(const __
     const int b = find_sequence((const int*)a.batch.cu_q, a.batch.batch, tok);
     if (b < 0) return;
     SeqRows r;
-    read_rows(a.batch, b, a.max_q, a.cache.page_size, &g_kv_status, r);
+    const uint32_t wrong = read_rows(a.batch, b, a.max_q, a.cache.page_size, r);
+    if (wrong) atomicOr(&g_kv_status, wrong);
     if ((int)tok >= r.first + r.n) return;
     const int own_end = a.causal ? max(0, r.len - r.n + ((int)tok - r.first) + 1) : r.len;
 
