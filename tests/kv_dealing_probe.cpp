@@ -1,6 +1,6 @@
 // The dealing of the attention kernel's work (csrc/kv_dealing.hpp), run on the host for random batches: every
-// (row tile, head, key tile) is taken exactly once; the warps that walk the tiles and the rows' warps see
-// the same order; what the joining kernel reads of a row is exactly what was written for it; every index
+// (row tile, head, key tile) is taken exactly once; loads, releases and first tiles are
+// marked where they belong; what the joining kernel reads of a row is exactly what was written for it; every index
 // stays inside its table or the workspace.
 //   kv_dealing_probe SEED CASES
 #include <cstdio>
@@ -113,54 +113,52 @@ int main(int argc, char** argv) {
                 }
                 REQUIRE(found == (left ? 1 : 0));
             }
-            // units in the walkers' order, by stream
-            std::vector<std::tuple<int, int, int, int, int>> by_stream[2], by_rows[2];    // list, b, tok, head, tile
+            // what the scheduling warp tells the others: units and rows' jobs
             Walk walk(d, pro);
             Job j;
-            int tile;
+            int tile, left[2] = {0, 0}, loaded = 0;
             bool use[2];
             while (walk.next(d, pro, j, tile, use[0], use[1])) {
                 ++tiles_seen;
                 REQUIRE(use[0] || use[1]);
-                REQUIRE(tile >= j.kt0 && tile < j.kt1 && tile * kTile < j.keys);
+                REQUIRE(tile >= j.kt0 && tile < j.kt1 && tile * kTile < j.keys && j.head < 65536);
                 const tsw_kv_pages& pg = j.own ? a.cache : a.prefix;
-                const int n = std::min(kTile, j.keys - tile * kTile), box = std::min((int)pg.page_size, kTile), first = tile * kTile / (int)pg.page_size;
-                const int last = first + (n + box - 1) / box - 1;
-                REQUIRE(last < (j.own ? width : ((int)a.prefix_len + page_size - 1) / page_size));
-                for (int s = 0; s < 2; ++s)
-                    if (use[s]) {
-                        const int tok = j.tok + (walk.pair && s ? (int)w.tile_tokens : 0);
-                        by_stream[s].push_back({j.own, j.b, tok, j.head, tile});
-                        REQUIRE(done.insert({j.own, tok, j.head, tile}).second);
-                    }
-            }
-            for (int s = 0; s < 2; ++s)
-                for (int own = 0; own < 2; ++own) {
-                    const bool pair = own ? w.own_pair : w.prefix_pair;
-                    Cursor cur(pro, pair ? 0 : s);
-                    while (cur.next(d, pro, own, j)) {
-                        const int seen = seen_by(j, pair, s), end = std::min(j.kt1, seen), tokens_here = pair && s ? j.n_b : j.n_a;
-                        const int tok = j.tok + (pair && s ? (int)w.tile_tokens : 0);
-                        for (int t = j.kt0; t < end; ++t) by_rows[s].push_back({own, j.b, tok, j.head, t});
-                        if (j.kt0 >= end) continue;
-                        REQUIRE(tokens_here >= 1 && tokens_here <= (int)w.tile_tokens && tok >= 0 && tok + tokens_here <= tokens);
-                        for (int i = 0; i < tokens_here * group; ++i) {
-                            const uint64_t row = (uint64_t)(tok + i / group) * a.q_heads + j.head * group + i % group;
-                            if (a.prefix_len == 0 && j.kt0 == 0 && end == seen) ++direct[row];
-                            else if (j.kt0 == 0) {
-                                const uint64_t h = home_index(d, own, row, a.q_heads);
+                for (int s = 0; s < 2; ++s) {
+                    if (!use[s]) continue;
+                    const Unit u = make_unit(j, tile, s, use[0], use[1]);
+                    const int n = unit_keys(u.flags), box = std::min((int)pg.page_size, kTile), first = tile * kTile / (int)pg.page_size;
+                    REQUIRE(n == std::min(kTile, j.keys - tile * kTile) && n >= 1 && unit_head(u.flags) == j.head);
+                    REQUIRE(first + (n + box - 1) / box - 1 < (j.own ? width : ((int)a.prefix_len + page_size - 1) / page_size));
+                    REQUIRE(((u.flags & kUnitStream) != 0) == (s == 1) && ((u.flags & kUnitOwn) != 0) == (j.own == 1));
+                    loaded += (u.flags & kUnitLoad) ? 1 : 0;
+                    REQUIRE(loaded == 1);                              // one load in front of the tile's units
+                    loaded -= (u.flags & kUnitRelease) ? 1 : 0;
+                    const RowJob r = make_row_job(d, j, walk.pair, s, cta);
+                    REQUIRE(((u.flags & kUnitFirst) != 0) == (left[s] == 0));
+                    if (u.flags & kUnitFirst) {
+                        left[s] = r.tiles;
+                        REQUIRE(r.tiles >= 1 && r.tokens >= 1 && r.tokens <= (int)w.tile_tokens && r.tok >= 0 && r.tok + r.tokens <= tokens);
+                        for (int i = 0; i < r.tokens * group; ++i) {
+                            const uint64_t row = (uint64_t)(r.tok + i / group) * a.q_heads + r.head * group + i % group;
+                            if (r.place == kPlaceDirect) ++direct[row];
+                            else if (r.place == kPlaceHome) {
+                                const uint64_t h = home_index(d, r.own, row, a.q_heads);
                                 REQUIRE(h < home_rows && home.insert(h).second);
                             } else {
-                                const uint64_t p = part_index(d, own, part_place(pair, range_index(d, pair, cta, s), s), i);
+                                const uint64_t p = part_index(d, r.own, r.place, i);
                                 REQUIRE(p < part_rows && part.insert(p).second);
                             }
                         }
                     }
+                    --left[s];
+                    REQUIRE(done.insert({j.own, r.tok, j.head, tile}).second);
                 }
-            for (int s = 0; s < 2; ++s) REQUIRE(by_stream[s] == by_rows[s]);
+                REQUIRE(loaded == 0);
+            }
+            REQUIRE(left[0] == 0 && left[1] == 0);
         }
         // ---- the joining kernel's view: every row of a sequence
-        size_t homes_read = 0, expected = 0;
+        size_t homes_read = 0;
         std::set<uint64_t> parts_read;
         for (int b = 0; b < batch; ++b) {
             SeqRows r;
@@ -205,7 +203,6 @@ int main(int argc, char** argv) {
                     }
                 }
         }
-        (void)expected;
         if (!wild && cu[0] == tok0 && tok1 == cu[batch]) {
             // nothing was written that nobody reads, except for rows of sequences longer than max_q
             bool all = true;

@@ -48,6 +48,7 @@ struct alignas(64) Params {
     tsw_prefix_attention_args a;
     Deal d;
     uint32_t* status;
+    int own_shift, prefix_shift;      // log2 of the page sizes
 };
 
 // ------------------------------------------------------------------ small PTX wrappers
@@ -75,21 +76,17 @@ __device__ __forceinline__ unsigned long long now() {
     return t;
 }
 // Every wait ends: after two seconds, or when another warp of the CTA has given up, it answers false, and the
-// caller leaves its loop.
-__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {
-    const unsigned long long t0 = now();
-    while (!mbar_try(bar, parity)) {
-        if (*gave_up) return false;
-        if (now() - t0 > kWaitNs) {
-            *gave_up = 1;
-            return false;
-        }
-    }
-    return true;
-}
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {     // a whole warp, one answer
+// caller leaves its loop.  A whole warp waits and gets one answer.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {
     if (__all_sync(~0u, mbar_try(bar, parity))) return true;
-    return __all_sync(~0u, wait_slow(bar, parity, gave_up));
+    const unsigned long long t0 = now();
+    bool ok;
+#pragma unroll 1
+    do {
+        ok = mbar_try(bar, parity);
+        if (!ok && now() - t0 > kWaitNs) *gave_up = 1;
+    } while (!__all_sync(~0u, ok) && !__any_sync(~0u, *gave_up));
+    return __all_sync(~0u, ok);
 }
 
 __device__ __forceinline__ void load_box4(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
@@ -124,10 +121,9 @@ __device__ __forceinline__ void tmem_ld32(uint32_t* r, uint32_t addr) {
                  "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                  : TSW_R8(r, 0), TSW_R8(r, 8), TSW_R8(r, 16), TSW_R8(r, 24) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
-                 "%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-                 ::"r"(addr), TSW_I8(r, 0), TSW_I8(r, 8), TSW_I8(r, 16), TSW_I8(r, 24) : "memory");
+__device__ __forceinline__ void tmem_ld16(uint32_t* r, uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : TSW_R8(r, 0), TSW_R8(r, 8) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -154,21 +150,35 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, f
 // bytes.  Q and K run along the head (the summed axis) in a row: eight-row groups lie 1024 bytes apart.
 // V's summed axis is its rows (keys): groups of eight keys lie 1024 bytes apart, and the next 64 head elements
 // a half (16 KB) further.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead_bytes) {
-    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lead_bytes >> 4) & 0x3fff) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+// The low word holds the address and the lead (units of 16 bytes): steps along a tile are added to it.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lead_bytes) { return addr >> 4 | lead_bytes >> 4 << 16; }
+__device__ __forceinline__ uint64_t desc(uint32_t lo) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(1024u >> 4 | 1u << 14 | 2u << 29));
+    return r;
 }
 
-struct Bars {                // mbarriers, byte addresses in shared memory
-    uint32_t k_full, k_empty, v_full, v_empty, q_full, q_empty, s_full, p_full, o_full;
+constexpr int kUnits = 16;                    // units on their way from the scheduling warp to the others
+constexpr int kJobs = 4;                      // rows' jobs on their way, per stream
+
+// mbarriers: byte offsets into the array in shared memory
+template <int kK, int kV> struct Bars {
+    static constexpr int k_full = 0, k_empty = k_full + 8 * kK, v_full = k_empty + 8 * kK, v_empty = v_full + 8 * kV, q_full = v_empty + 8 * kV,
+                         s_full = q_full + 16, o_full = s_full + 16, unit_full = o_full + 16, job_full = unit_full + 8 * kUnits,
+                         ones = (job_full + 16 * kJobs) / 8,                          // up to here one arrival completes a phase
+                         unit_empty = 8 * ones, p_full = unit_empty + 8 * kUnits, job_empty = p_full + 16, bytes = job_empty + 16 * kJobs;
 };
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __grid_constant__ Params p) {
     using S = Shape<DP>;
+    using B = Bars<S::kK, S::kV>;
     constexpr int kHalves = DP / 64;
     constexpr uint32_t kHalfBytes = kTile * 128;
     extern __shared__ uint8_t s_raw[];
-    __shared__ __align__(8) uint64_t s_bars[2 * (S::kK + S::kV) + 10];
+    __shared__ __align__(8) uint64_t s_bars[B::bytes / 8];
+    __shared__ Unit s_units[kUnits];
+    __shared__ RowJob s_jobs[2][kJobs];
     __shared__ Prologue s_pro;
     __shared__ uint32_t s_tmem, s_scan[kThreads / 32];
     __shared__ uint32_t s_gave_up;
@@ -177,84 +187,79 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
     const tsw_prefix_attention_args& a = p.a;
     const Deal& d = p.d;
     const AttentionLayout& w = d.w;
-    const int group = w.group, tile_tokens = w.tile_tokens;
-    uint8_t* ws = (uint8_t*)a.workspace;
+    const uint32_t bar = smem_addr(s_bars);
+    const uint32_t q_at = (smem_addr(s_raw) + 1023) & ~1023u, k_at = q_at + 2 * S::kTileBytes, v_at = k_at + S::kK * S::kTileBytes;
 
-    const uint32_t tiles = (smem_addr(s_raw) + 1023) & ~1023u;
-    const uint32_t q_at = tiles, k_at = q_at + 2 * S::kTileBytes, v_at = k_at + S::kK * S::kTileBytes;
-    Bars bar;
-    {
-        const uint32_t b = smem_addr(s_bars);
-        bar.k_full = b;
-        bar.k_empty = bar.k_full + 8 * S::kK;
-        bar.v_full = bar.k_empty + 8 * S::kK;
-        bar.v_empty = bar.v_full + 8 * S::kV;
-        bar.q_full = bar.v_empty + 8 * S::kV;
-        bar.q_empty = bar.q_full + 16;
-        bar.s_full = bar.q_empty + 16;
-        bar.p_full = bar.s_full + 16;
-        bar.o_full = bar.p_full + 16;
-    }
-    if (tid == 0) {
-        for (int i = 0; i < 2 * S::kK + 2 * S::kV + 6; ++i) mbar_init(bar.k_full + 8 * i, 1);
-        mbar_init(bar.p_full, 4);
-        mbar_init(bar.p_full + 8, 4);
-        mbar_init(bar.o_full, 1);
-        mbar_init(bar.o_full + 8, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        s_gave_up = 0;
-        s_pro.own[0].left = s_pro.own[1].left = 0;
+    // ---- where this CTA's ranges begin: every CTA sums the tiles of all sequences
+    const uint32_t batch = a.batch.batch, each = (batch + kThreads - 1) / kThreads;
+    const uint32_t b_lo = min(batch, tid * each), b_hi = min(batch, b_lo + each);
+    uint32_t mine = 0, wrong = 0;
+#pragma unroll 1
+    for (uint32_t b = b_lo; b < b_hi; ++b) {
+        SeqRows r;
+        wrong |= read_rows(a.batch, b, a.max_q, a.cache.page_size, r);
+        mine += sequence_tiles(d, r);
     }
     if (warp == 10) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-
-    // ---- where this CTA's ranges begin: every CTA sums the tiles of all sequences
-    const uint32_t batch = a.batch.batch, each = (batch + kThreads - 1) / kThreads;
-    const uint32_t b_lo = min(batch, tid * each), b_hi = min(batch, b_lo + each);
-    SeqRows r;
-    uint32_t mine = 0, wrong = 0;
-    for (uint32_t b = b_lo; b < b_hi; ++b) {
-        wrong |= read_rows(a.batch, b, a.max_q, a.cache.page_size, r);
-        mine += sequence_tiles(d, r);
+    if (warp == 9) {
+        for (int i = lane; i < B::bytes / 8; i += 32)
+            mbar_init(bar + 8 * i, i < B::ones ? 1 : i < B::p_full / 8 ? 3 : 4);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8 && lane < 6) {
+        const CUtensorMap* map = &p.q_prefix + lane;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+    }
+    if (tid == 0) {
+        s_gave_up = 0;
+        s_pro.own[0].left = s_pro.own[1].left = 0;
     }
     if (wrong && blockIdx.x == 0) atomicOr(p.status, wrong);
-    uint32_t incl = mine;
+    uint32_t before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(~0u, incl, o);
-        if (lane >= o) incl += up;
+        const uint32_t up = __shfl_up_sync(~0u, before, o);
+        if (lane >= o) before += up;
     }
-    if (lane == 31) s_scan[warp] = incl;
+    if (lane == 31) s_scan[warp] = before;
+    before -= mine;
     __syncthreads();
-    uint32_t before = incl - mine, total = 0;
+    uint32_t total = 0;
+#pragma unroll
     for (int i = 0; i < kThreads / 32; ++i) {
-        if (i < warp) before += s_scan[i];
+        if (i == warp) before += total;
         total += s_scan[i];
     }
-    int tok0, tok1;
-    const uint32_t rts = prefix_rows(d, tok0, tok1);
-    const uint32_t prefix_total = a.kv_heads * rts * w.prefix_tiles;
-    if (tid < 2) s_pro.prefix[tid] = range_at(d, w.prefix_pair, prefix_total, blockIdx.x, tid);
-    if (tid == 0) {
-        s_pro.prefix_rt = max(1u, rts);
-        s_pro.tok0 = tok0;
-        s_pro.tok1 = tok1;
+    if (warp == 11) {
+        int tok0, tok1;
+        const uint32_t rts = prefix_rows(d, tok0, tok1), prefix_total = a.kv_heads * rts * w.prefix_tiles;
+        if (lane < 2) s_pro.prefix[lane] = range_at(d, w.prefix_pair, prefix_total, blockIdx.x, lane);
+        if (lane == 0) {
+            s_pro.prefix_rt = max(1u, rts);
+            s_pro.tok0 = tok0;
+            s_pro.tok1 = tok1;
+            if (blockIdx.x == 0) {                    // for the joining kernel
+                uint32_t* base = (uint32_t*)((uint8_t*)a.workspace + w.own_base);
+                base[batch] = total;
+                base[batch + 1] = prefix_total;
+            }
+        }
     }
-    if (blockIdx.x == 0) {                        // for the joining kernel
-        uint32_t* base = (uint32_t*)(ws + w.own_base);
+    if (blockIdx.x == 0) {
+        uint32_t* base = (uint32_t*)((uint8_t*)a.workspace + w.own_base);
         uint32_t at = before;
+#pragma unroll 1
         for (uint32_t b = b_lo; b < b_hi; ++b) {
             base[b] = at;
+            SeqRows r;
             read_rows(a.batch, b, a.max_q, a.cache.page_size, r);
             at += sequence_tiles(d, r);
         }
-        if (tid == 0) {
-            base[batch] = total;
-            base[batch + 1] = prefix_total;
-        }
     }
+#pragma unroll 1
     for (int s = 0; s < 2; ++s) {
         const Range g = range_at(d, w.own_pair, total, blockIdx.x, s);
         if (g.end > g.x && g.x >= before && g.x < before + mine) find_start(d, b_lo, b_hi, g.x - before, g.end - g.x, s_pro.own[s]);
@@ -265,307 +270,328 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = s_tmem;
 
-    if (warp == 8 || warp == 9) {
-        // ---------------------------------------------------------------- keys (8) and values (9)
-        const bool is_v = warp == 9;
-        const int stages = is_v ? S::kV : S::kK;
-        const uint32_t at = is_v ? v_at : k_at, full = is_v ? bar.v_full : bar.k_full, empty = is_v ? bar.v_empty : bar.k_empty;
-        const CUtensorMap* maps[2] = {is_v ? &p.v_prefix : &p.k_prefix, is_v ? &p.v_own : &p.k_own};
-        Walk walk(d, s_pro);
-        Job j;
-        int tile, slot = 0;
-        uint32_t phase = 0, issued = 0;
-        bool u0, u1;
-        while (walk.next(d, s_pro, j, tile, u0, u1)) {
-            const tsw_kv_pages& pg = j.own ? a.cache : a.prefix;
-            const int* table = j.own ? (const int*)a.batch.page_table + (uint64_t)j.b * a.batch.table_stride : (const int*)a.prefix_table;
-            const int ps = pg.page_size, key0 = tile * kTile, n = min(kTile, j.keys - key0);
-            const int box = min(ps, kTile), boxes = (n + box - 1) / box, first = key0 / ps, in_page = key0 - first * ps;
-            int page = lane < boxes ? table[first + lane] : 0;        // before the wait: its latency passes under it
-            if (!wait(empty + 8 * slot, phase ^ 1, gave_up)) break;
-            if (lane == 0) mbar_expect(full + 8 * slot, boxes * box * 128 * kHalves);
-            __syncwarp();
-            for (int i = lane; i < boxes; i += 32) {
-                if (i >= 32) page = table[first + i];
-                // a number outside the cache is recorded; the copy unit fills such a box with zeros
-                if ((uint32_t)page >= pg.pages) { atomicOr(p.status, TSW_KV_BAD_PAGE); page = pg.pages; }
-                const uint32_t dst = at + slot * S::kTileBytes + i * box * 128;
-#pragma unroll
-                for (int h = 0; h < kHalves; ++h)
-                    load_box4(dst + h * kHalfBytes, maps[j.own], h * 64, in_page, j.head, page, full + 8 * slot);
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        if (warp == 11) {
+            // ------------------------------------------------------------ scheduling
+            Walk walk(d, s_pro);
+            Job j;
+            int tile;
+            uint32_t n = 0, jobs[2] = {0, 0};
+            bool use[2], ok = true;
+#pragma unroll 1
+            while (ok) {
+                const bool more = walk.next(d, s_pro, j, tile, use[0], use[1]);
+                if (!more) use[0] = use[1] = true;
+#pragma unroll 1
+                for (int s = 0; s < 2 && ok; ++s) {
+                    if (s ? !use[1] : !use[0]) continue;
+                    if (!more || tile == j.kt0) {                     // also tells both streams' rows of the end
+                        const uint32_t i = s ? jobs[1]++ : jobs[0]++, at = s * kJobs + i % kJobs;
+                        ok = wait(bar + B::job_empty + 8 * at, (i / kJobs & 1) ^ 1, gave_up);
+                        if (!ok) break;
+                        if (lane == 0) {
+                            RowJob r = {};
+                            if (more) r = make_row_job(d, j, walk.pair, s, blockIdx.x);
+                            s_jobs[s][i % kJobs] = r;
+                            mbar_arrive(bar + B::job_full + 8 * at);
+                        }
+                        if (!more && s == 0) continue;
+                    }
+                    ok = wait(bar + B::unit_empty + 8 * (n % kUnits), (n / kUnits & 1) ^ 1, gave_up);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        s_units[n % kUnits] = more ? make_unit(j, tile, s, use[0], use[1]) : Unit{kUnitEnd, 0, 0, 0};
+                        mbar_arrive(bar + B::unit_full + 8 * (n % kUnits));
+                    }
+                    ++n;
+                }
+                if (!more) break;
             }
-            ++issued;
-            if (++slot == stages) { slot = 0; phase ^= 1; }
-        }
-        if (*gave_up)        // copies in flight land before the CTA ends
-            for (int i = 0; i < stages && i < (int)issued; ++i) {
-                const unsigned long long t0 = now();
-                const uint32_t last = (i < slot) ? phase : phase ^ 1;
-                while (!mbar_try(full + 8 * i, last) && now() - t0 < kWaitNs / 8) {}
-            }
-    } else if (warp == 11) {
-        // ---------------------------------------------------------------- queries
-        Walk walk(d, s_pro);
-        Job j;
-        int tile;
-        uint32_t count[2] = {0, 0};
-        bool use[2];
-        while (walk.next(d, s_pro, j, tile, use[0], use[1])) {
-            if (tile != j.kt0) continue;
-            bool ok = true;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (!use[s] || !ok) continue;
-                ok = wait(bar.q_empty + 8 * s, (count[s] & 1) ^ 1, gave_up);
-                if (!ok) break;
-                ++count[s];
-                if (lane == 0) {
-                    const uint32_t box = j.own ? w.own_box_tokens : w.tile_tokens;
-                    const int tok = j.tok + (walk.pair && s ? tile_tokens : 0);
-                    mbar_expect(bar.q_full + 8 * s, box * group * 128 * kHalves);
+        } else if (warp < 10) {
+            // ------------------------------------------------------------ keys (8) and values (9)
+            const bool is_v = warp == 9;
+            const int stages = is_v ? S::kV : S::kK;
+            const uint32_t at = is_v ? v_at : k_at, full = bar + (is_v ? B::v_full : B::k_full), empty = bar + (is_v ? B::v_empty : B::k_empty);
+            int slot = 0;
+            uint32_t phase = 0, issued = 0;
+#pragma unroll 1
+            for (uint32_t n = 0;; ++n) {
+                if (!wait(bar + B::unit_full + 8 * (n % kUnits), n / kUnits & 1, gave_up)) break;
+                const Unit u = s_units[n % kUnits];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar + B::unit_empty + 8 * (n % kUnits));
+                if (u.flags & kUnitEnd) break;
+                if (!(u.flags & kUnitLoad)) continue;
+                const bool own = u.flags & kUnitOwn;
+                const tsw_kv_pages& pg = own ? a.cache : a.prefix;
+                const CUtensorMap* map = own ? (is_v ? &p.v_own : &p.k_own) : (is_v ? &p.v_prefix : &p.k_prefix);
+                const int shift = own ? p.own_shift : p.prefix_shift, box = min(1 << shift, kTile);
+                const int boxes = (unit_keys(u.flags) + box - 1) / box, first = u.tile * kTile >> shift, in_page = u.tile * kTile & ((1 << shift) - 1);
+                const int* table = (own ? (const int*)a.batch.page_table + (uint64_t)u.b * a.batch.table_stride : (const int*)a.prefix_table) + first;
+                int page = lane < boxes ? table[lane] : 0;                // before the wait: its latency passes under it
+                if (!wait(empty + 8 * slot, phase ^ 1, gave_up)) break;
+                if (lane == 0) mbar_expect(full + 8 * slot, boxes * box * 128 * kHalves);
+                __syncwarp();
+#pragma unroll 1
+                for (int i = lane; i < boxes; i += 32) {
+                    if (i >= 32) page = table[i];
+                    // a number outside the cache is recorded; the copy unit fills such a box with zeros
+                    if ((uint32_t)page >= pg.pages) { atomicOr(p.status, TSW_KV_BAD_PAGE); page = pg.pages; }
+                    const uint32_t dst = at + slot * S::kTileBytes + i * box * 128;
 #pragma unroll
                     for (int h = 0; h < kHalves; ++h)
-                        load_box3(q_at + s * S::kTileBytes + h * kHalfBytes, j.own ? &p.q_own : &p.q_prefix, h * 64, j.head * group, tok,
-                                  bar.q_full + 8 * s);
+                        load_box4(dst + h * kHalfBytes, map, h * 64, in_page, unit_head(u.flags), page, full + 8 * slot);
                 }
+                ++issued;
+                if (++slot == stages) { slot = 0; phase ^= 1; }
             }
-            if (!ok) break;
-        }
-        if (*gave_up)
-            for (int s = 0; s < 2; ++s)
-                if (count[s]) {
+            if (*gave_up)        // copies in flight land before the CTA ends
+                for (int i = 0; i < stages && i < (int)issued; ++i) {
                     const unsigned long long t0 = now();
-                    while (!mbar_try(bar.q_full + 8 * s, (count[s] - 1) & 1) && now() - t0 < kWaitNs / 8) {}
+                    while (!mbar_try(full + 8 * i, i < slot ? phase : phase ^ 1) && now() - t0 < kWaitNs / 8) {}
                 }
-    } else if (warp == 10) {
-        // ---------------------------------------------------------------- products
-        // Order: S of a tile, then the O product of the tile before it, whose exponentials ran meanwhile.
-        constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u << 7 | 1u << 10;
-        constexpr uint32_t kDescS = 1u << 4 | kType | (kTile / 8) << 17 | (kTile / 16) << 24;
-        constexpr uint32_t kDescO = 1u << 4 | kType | 1u << 16 | (DP / 8) << 17 | (kTile / 16) << 24;
-        Walk walk(d, s_pro);
-        Job j;
-        int tile, k_slot = 0, v_slot = 0;
-        uint32_t k_phase = 0, v_phase = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
-        struct Pending { bool any = false, first, load, release; int s, slot, keys; uint32_t phase; } pend;
-        bool use[2], ok = true;
-
-        auto product_o = [&]() {
-            const Pending& u = pend;
-            if (u.load) ok = wait(bar.v_full + 8 * u.slot, u.phase, gave_up);
-            const uint32_t v = v_at + u.slot * S::kTileBytes;
-            const int steps = (u.keys + 15) / 16;
-            if (u.load && ok && (u.keys & 15)) {
-                // Rows behind the last key hold whatever their page holds, and a weight of zero does not
-                // silence an infinity: clear what the last step would read.
-                const int rows = steps * 16 - u.keys;
-                for (int i = lane; i < rows * 8 * kHalves; i += 32) {
-                    const uint32_t at = v + (i / (rows * 8)) * kHalfBytes + (u.keys + (i / 8) % rows) * 128 + (i % 8) * 16;
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        } else {
+            // ------------------------------------------------------------ products
+            // Order: S of a unit, then the O product of the unit before it, whose exponentials ran meanwhile.  When both
+            // are one stream's, O goes first: S would overwrite the weights.
+            constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u << 7 | 1u << 10;
+            constexpr uint32_t kDescS = 1u << 4 | kType | (kTile / 8) << 17 | (kTile / 16) << 24;
+            constexpr uint32_t kDescO = 1u << 4 | kType | 1u << 16 | (DP / 8) << 17 | (kTile / 16) << 24;
+            uint32_t n_q = 0, n_p = 0;                    // phases of both streams, bit s
+            int k_slot = 0, v_slot = 0, old_v_slot = 0;
+            uint32_t k_phase = 0, v_phase = 0, old_v_phase = 0, old = kUnitEnd;
+            bool ok = true;
+#pragma unroll 1
+            for (uint32_t n = 0; ok; ++n) {
+                ok = wait(bar + B::unit_full + 8 * (n % kUnits), n / kUnits & 1, gave_up);
+                if (!ok) break;
+                const uint32_t flags = s_units[n % kUnits].flags;
                 __syncwarp();
-            }
-            ok = ok && wait(bar.p_full + 8 * u.s, n_p[u.s]++ & 1, gave_up);
-            if (!ok) return;
-            fence_after();
-            if (lane == 0) {
-                const uint32_t base = tmem + u.s * 256;
-                for (int k = 0; k < steps; ++k)
-                    mma_ts(base + 128, base + k * 8, smem_desc(v + k * 2048, kHalfBytes), kDescO, !(u.first && k == 0));
-                mma_commit(bar.o_full + 8 * u.s);
-                if (u.release) mma_commit(bar.v_empty + 8 * u.slot);
-            }
-            __syncwarp();
-            pend.any = false;
-        };
-
-        while (ok && walk.next(d, s_pro, j, tile, use[0], use[1])) {
-            ok = wait(bar.k_full + 8 * k_slot, k_phase, gave_up);
-            bool load = true;
+                if (lane == 0) mbar_arrive(bar + B::unit_empty + 8 * (n % kUnits));
+                const bool same = !((flags ^ old) & kUnitStream);
+#pragma unroll 1
+                for (int step = 0; step < 2 && ok; ++step) {
+                    if ((step == 0) == same) {
+                        if (old & kUnitEnd) continue;
+                        const int s = old & kUnitStream, keys = unit_keys(old), steps = (keys + 15) / 16;
+                        const uint32_t v = v_at + old_v_slot * S::kTileBytes;
+                        if (old & kUnitLoad) {
+                            ok = wait(bar + B::v_full + 8 * old_v_slot, old_v_phase, gave_up);
+                            if (ok && (keys & 15)) {
+                                // Rows behind the last key hold whatever their page holds, and a weight of zero
+                                // does not silence an infinity: clear what the last step would read.
+                                const int rows = steps * 16 - keys;
+#pragma unroll 1
+                                for (int i = lane; i < rows * 8 * kHalves; i += 32) {
+                                    const uint32_t to = v + (i / (rows * 8)) * kHalfBytes + (keys + (i / 8) % rows) * 128 + (i % 8) * 16;
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
+                                }
+                                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                                __syncwarp();
+                            }
+                        }
+                        ok = ok && wait(bar + B::p_full + 8 * s, n_p >> s & 1, gave_up);
+                        if (!ok) break;
+                        n_p ^= 1u << s;
+                        fence_after();
+                        if (lane == 0) {
+                            const uint32_t base = tmem + s * 256, v_lo = desc_lo(v, kHalfBytes);
+                            mma_ts(base + 128, base, desc(v_lo), kDescO, !(old & kUnitFirst));
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (!use[s] || !ok) continue;
-                if (pend.any && pend.s == s) product_o();
-                if (!ok) break;
-                const bool first = tile == j.kt0, ends = tile + 1 == min(j.kt1, seen_by(j, walk.pair, s));
-                const bool release = s == 1 || !use[1];
-                if (first) ok = wait(bar.q_full + 8 * s, n_q[s]++ & 1, gave_up);
-                if (!ok) break;
-                fence_after();
-                if (lane == 0) {
-                    const uint32_t q = q_at + s * S::kTileBytes, k = k_at + k_slot * S::kTileBytes;
+                            for (int k = 1; k < kTile / 16; ++k)
+                                if (k < steps) mma_ts(base + 128, base + k * 8, desc(v_lo + (k * 2048 >> 4)), kDescO, true);
+                            mma_commit(bar + B::o_full + 8 * s);
+                            if (old & kUnitRelease) mma_commit(bar + B::v_empty + 8 * old_v_slot);
+                        }
+                        __syncwarp();
+                    } else {
+                        if (flags & kUnitEnd) continue;
+                        const int s = flags & kUnitStream;
+                        if (flags & kUnitLoad) ok = wait(bar + B::k_full + 8 * k_slot, k_phase, gave_up);
+                        if (ok && (flags & kUnitFirst)) {
+                            ok = wait(bar + B::q_full + 8 * s, n_q >> s & 1, gave_up);
+                            n_q ^= 1u << s;
+                        }
+                        if (!ok) break;
+                        fence_after();
+                        if (lane == 0) {
+                            const uint32_t q_lo = desc_lo(q_at + s * S::kTileBytes, 16), k_lo = desc_lo(k_at + k_slot * S::kTileBytes, 16);
 #pragma unroll
-                    for (int i = 0; i < DP / 16; ++i) {
-                        const uint32_t off = (i / 4) * kHalfBytes + (i % 4) * 32;
-                        mma_ss(tmem + s * 256, smem_desc(q + off, 16), smem_desc(k + off, 16), kDescS, i > 0);
+                            for (int i = 0; i < DP / 16; ++i) {
+                                const uint32_t off = ((i / 4) * kHalfBytes + (i % 4) * 32) >> 4;
+                                mma_ss(tmem + s * 256, desc(q_lo + off), desc(k_lo + off), kDescS, i > 0);
+                            }
+                            mma_commit(bar + B::s_full + 8 * s);
+                            if (flags & kUnitRelease) mma_commit(bar + B::k_empty + 8 * k_slot);
+                        }
+                        __syncwarp();
                     }
-                    mma_commit(bar.s_full + 8 * s);
-                    if (release) mma_commit(bar.k_empty + 8 * k_slot);
-                    if (ends) mma_commit(bar.q_empty + 8 * s);
                 }
-                __syncwarp();
-                if (pend.any) product_o();
-                if (!ok) break;
-                pend.any = true;
-                pend.first = first;
-                pend.load = load;
-                pend.release = release;
-                pend.s = s;
-                pend.slot = v_slot;
-                pend.phase = v_phase;
-                pend.keys = min(kTile, j.keys - tile * kTile);
-                load = false;
+                if (flags & kUnitEnd) break;
+                old = flags;
+                old_v_slot = v_slot;
+                old_v_phase = v_phase;
+                if (flags & kUnitRelease) {
+                    if (++k_slot == S::kK) { k_slot = 0; k_phase ^= 1; }
+                    if (++v_slot == S::kV) { v_slot = 0; v_phase ^= 1; }
+                }
             }
-            if (++k_slot == S::kK) { k_slot = 0; k_phase ^= 1; }
-            if (++v_slot == S::kV) { v_slot = 0; v_phase ^= 1; }
         }
-        if (ok && pend.any) product_o();
     } else {
         // ---------------------------------------------------------------- rows: one thread each
-        const int s = warp >> 2, row = tid & 127;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        const int s = warp >> 2, row = tid & 127, group = w.group;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;                 // this warp's quarter of the tensor memory's lanes
         const uint32_t t_s = tmem + lanes + s * 256, t_o = t_s + 128;
+        const uint32_t b_s = bar + B::s_full + 8 * s, b_p = bar + B::p_full + 8 * s, b_o = bar + B::o_full + 8 * s;
+        const uint32_t b_jf = bar + B::job_full + 8 * kJobs * s, b_je = bar + B::job_empty + 8 * kJobs * s;
         const float c = a.scale * 1.4426950408889634f;
         const int tok_in_tile = row / group, head_in_group = row - tok_in_tile * group;
-        uint32_t count = 0;
+        const bool loads_q = (warp & 3) == 0;                             // the warp that fetches the stream's queries
+        uint32_t count = 0, asked = 0;                                    // units so far; jobs whose queries are on their way
+        auto load_q = [&](uint32_t i) {                                   // of job i, which has been read or seen to be there
+            const RowJob& j = s_jobs[s][i % kJobs];
+            if (lane == 0 && j.tiles) {
+                const uint32_t box = j.own ? w.own_box_tokens : w.tile_tokens, to = q_at + s * S::kTileBytes;
+                const CUtensorMap* map = j.own ? &p.q_own : &p.q_prefix;
+                mbar_expect(bar + B::q_full + 8 * s, box * group * 128 * kHalves);
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h) load_box3(to + h * kHalfBytes, map, h * 64, j.head * group, j.tok, bar + B::q_full + 8 * s);
+            }
+            asked = i + 1;
+        };
         bool ok = true;
-        for (int own = 0; own < 2 && ok; ++own) {
-            const bool pair = own ? w.own_pair : w.prefix_pair;
-            Cursor cur(s_pro, pair ? 0 : s);
-            Job j;
-            while (ok && cur.next(d, s_pro, own, j)) {
-                const int seen = seen_by(j, pair, s), end = min(j.kt1, seen);
-                const int tokens = pair && s ? j.n_b : j.n_a, tok = j.tok + (pair && s ? tile_tokens : 0) + tok_in_tile;
-                const bool mine = tok_in_tile < tokens;
-                const bool warp_on = (warp & 3) * 32 < tokens * group;
-                const int visible = min(j.keys, max(0, j.limit + tok + 1));     // keys this row sees, from the segment's start
-                float top = -INFINITY, sum = 0.f;
-                for (int tile = j.kt0; tile < end; ++tile, ++count) {
-                    ok = wait(bar.s_full + 8 * s, count & 1, gave_up);
-                    if (!ok) break;
-                    fence_after();
-                    if (warp_on) {
-                        const int left = visible - tile * kTile;                // of this tile
-                        const int chunks = (min(kTile, j.keys - tile * kTile) + 31) / 32;
-                        float x[kTile];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (i < chunks) tmem_ld32((uint32_t*)x + 32 * i, t_s + 32 * i);
-                        tmem_wait_ld();
-                        if (__any_sync(~0u, left < chunks * 32)) {
-#pragma unroll
-                            for (int i = 0; i < kTile; ++i)
-                                if (i >= left) x[i] = -INFINITY;
-                        }
-                        float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (i < chunks) {
-#pragma unroll
-                                for (int e = 0; e < 32; e += 4) {
-                                    m0 = fmaxf(m0, x[32 * i + e]);
-                                    m1 = fmaxf(m1, x[32 * i + e + 1]);
-                                    m2 = fmaxf(m2, x[32 * i + e + 2]);
-                                    m3 = fmaxf(m3, x[32 * i + e + 3]);
-                                }
-                            }
-                        const float here = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-                        if (tile == j.kt0) {
-                            top = here;
-                        } else {
-                            const bool grow = (here - top) * c > kGrow;          // also from -inf; never between two of them
-                            if (__any_sync(~0u, grow)) {
-                                const float f = grow ? exp2_fast((top - here) * c) : 1.f;
-                                if (grow) top = here;
-                                sum *= f;
-                                ok = wait(bar.o_full + 8 * s, (count - 1) & 1, gave_up);
-                                if (!ok) break;
-                                fence_after();
-#pragma unroll
-                                for (int i = 0; i < DP / 32; ++i) {
-                                    float o[32];
-                                    tmem_ld32((uint32_t*)o, t_o + 32 * i);
-                                    tmem_wait_ld();
-#pragma unroll
-                                    for (int e = 0; e < 32; ++e) o[e] *= f;
-                                    tmem_st32(t_o + 32 * i, (uint32_t*)o);
-                                }
-                            }
-                        }
-                        const float base = top == -INFINITY ? 0.f : top * c;
-                        float p0 = 0.f, p1 = 0.f, p2 = 0.f, p3 = 0.f;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (i < chunks) {
-                                uint32_t packed[16];
-#pragma unroll
-                                for (int e = 0; e < 32; e += 4) {
-                                    const float e0 = exp2_fast(fmaf(x[32 * i + e], c, -base)), e1 = exp2_fast(fmaf(x[32 * i + e + 1], c, -base));
-                                    const float e2 = exp2_fast(fmaf(x[32 * i + e + 2], c, -base)), e3 = exp2_fast(fmaf(x[32 * i + e + 3], c, -base));
-                                    p0 += e0; p1 += e1; p2 += e2; p3 += e3;
-                                    packed[e / 2] = pack2<T>(e0, e1);
-                                    packed[e / 2 + 1] = pack2<T>(e2, e3);
-                                }
-                                tmem_st16(t_s + 16 * i, packed);
-                            }
-                        sum += (p0 + p1) + (p2 + p3);
-                        tmem_wait_st();
-                    }
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar.p_full + 8 * s);
-                }
-                if (!ok || j.kt0 >= end) continue;
-                // ---- the range's result: into the output when it is all there is, else by row (an item's first
-                // range) or by stream (one that continues)
-                ok = wait(bar.o_full + 8 * s, (count - 1) & 1, gave_up);
+#pragma unroll 1
+        for (uint32_t i = 0; ok; ++i) {
+            ok = wait(b_jf + 8 * (i % kJobs), i / kJobs & 1, gave_up);
+            if (!ok) break;
+            if (loads_q && asked == i) load_q(i);
+            const RowJob j = s_jobs[s][i % kJobs];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_je + 8 * (i % kJobs));
+            if (!j.tiles) break;
+            const int tok = j.tok + tok_in_tile;
+            const bool warp_on = (warp & 3) * 32 < j.tokens * group;
+            int left = min(j.keys, max(0, j.limit + tok));                // keys this row sees from here on
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll 1
+            for (int tile = 0; tile < j.tiles; ++tile, ++count, left -= kTile) {
+                ok = wait(b_s, count & 1, gave_up);
                 if (!ok) break;
                 fence_after();
-                if (!warp_on) continue;
-                const bool direct = a.prefix_len == 0 && j.kt0 == 0 && end == seen;
-                const uint32_t head = j.head * group + head_in_group;
-                float* dst = nullptr;
-                float2* ml = nullptr;
-                uint8_t* out = nullptr;
-                float inv = 0.f;
-                if (mine) {
-                    const uint64_t row_at = (uint64_t)tok * a.q_heads + head;
-                    if (direct) {
-                        out = (uint8_t*)(a.out + (uint64_t)tok * a.out_token_stride + (uint64_t)head * a.out_head_stride);
-                        inv = sum == 0.f ? 0.f : 1.f / sum;
-                        if (a.lse) ((float*)a.lse)[row_at] = sum == 0.f ? -INFINITY : (top * c + log2f(sum)) * 0.6931471805599453f;
-                    } else if (j.kt0 == 0) {
-                        const uint64_t at = home_index(d, own, row_at, a.q_heads);
-                        dst = (float*)(ws + w.home_o) + at * a.head_dim;
-                        ml = (float2*)(ws + w.home_ml) + at;
-                    } else {
-                        const uint64_t at = part_index(d, own, part_place(pair, range_index(d, pair, blockIdx.x, s), s), row);
-                        dst = (float*)(ws + w.part_o) + at * a.head_dim;
-                        ml = (float2*)(ws + w.part_ml) + at;
-                    }
-                    if (ml) *ml = make_float2(top == -INFINITY ? -INFINITY : top * c, sum);
-                }
+                // The job's last S is there, so its queries are done with: fetch the next job's, if it is known yet.
+                if (loads_q && tile == j.tiles - 1 && __all_sync(~0u, mbar_try(b_jf + 8 * ((i + 1) % kJobs), (i + 1) / kJobs & 1))) load_q(i + 1);
+                if (warp_on) {
+                    float x[kTile];
 #pragma unroll
-                for (int i = 0; i < DP / 32; ++i) {
-                    float o[32];
-                    tmem_ld32((uint32_t*)o, t_o + 32 * i);
+                    for (int k = 0; k < 4; ++k) tmem_ld32((uint32_t*)x + 32 * k, t_s + 32 * k);
                     tmem_wait_ld();
-                    if (out) {
+                    if (__any_sync(~0u, left < kTile)) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8)
-                            if (32 * i + e < (int)a.head_dim)
-                                *(uint4*)(out + 2 * (32 * i + e)) =
-                                    make_uint4(pack2<T>(o[e] * inv, o[e + 1] * inv), pack2<T>(o[e + 2] * inv, o[e + 3] * inv),
-                                               pack2<T>(o[e + 4] * inv, o[e + 5] * inv), pack2<T>(o[e + 6] * inv, o[e + 7] * inv));
-                    } else if (dst) {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            if (32 * i + e < (int)a.head_dim) *(float4*)(dst + 32 * i + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        for (int k = 0; k < kTile; ++k)
+                            if (k >= left) x[k] = -INFINITY;
                     }
+                    float m0 = x[0], m1 = x[1], m2 = x[2], m3 = x[3];
+#pragma unroll
+                    for (int k = 4; k < kTile; k += 4) {
+                        m0 = fmaxf(m0, x[k]);
+                        m1 = fmaxf(m1, x[k + 1]);
+                        m2 = fmaxf(m2, x[k + 2]);
+                        m3 = fmaxf(m3, x[k + 3]);
+                    }
+                    const float here = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+                    if (tile == 0) {
+                        top = here;
+                    } else {
+                        const bool grow = (here - top) * c > kGrow;              // also from -inf; never between two of them
+                        if (__any_sync(~0u, grow)) {
+                            const float f = grow ? exp2_fast((top - here) * c) : 1.f;
+                            if (grow) top = here;
+                            sum *= f;
+                            ok = wait(b_o, (count - 1) & 1, gave_up);
+                            if (!ok) break;
+                            fence_after();
+#pragma unroll 1
+                            for (int k = 0; k < DP; k += 16) {
+                                float o[16];
+                                tmem_ld16((uint32_t*)o, t_o + k);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) o[e] *= f;
+                                tmem_st16(t_o + k, (uint32_t*)o);
+                            }
+                        }
+                    }
+                    const float base = top == -INFINITY ? 0.f : top * c;
+                    float p0 = 0.f, p1 = 0.f, p2 = 0.f, p3 = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t packed[16];
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            const float e0 = exp2_fast(fmaf(x[32 * k + e], c, -base)), e1 = exp2_fast(fmaf(x[32 * k + e + 1], c, -base));
+                            const float e2 = exp2_fast(fmaf(x[32 * k + e + 2], c, -base)), e3 = exp2_fast(fmaf(x[32 * k + e + 3], c, -base));
+                            p0 += e0;
+                            p1 += e1;
+                            p2 += e2;
+                            p3 += e3;
+                            packed[e / 2] = pack2<T>(e0, e1);
+                            packed[e / 2 + 1] = pack2<T>(e2, e3);
+                        }
+                        tmem_st16(t_s + 16 * k, packed);
+                    }
+                    sum += (p0 + p1) + (p2 + p3);
+                    tmem_wait_st();
                 }
                 fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b_p);
             }
+            if (!ok) break;
+            // ---- the range's result: into the output when it is all there is, else by row (an item's first
+            // range) or by stream (one that continues)
+            ok = wait(b_o, (count - 1) & 1, gave_up);
+            if (!ok) break;
+            fence_after();
+            if (!warp_on) continue;
+            uint8_t* out = nullptr;
+            float f = 1.f;
+            if (tok_in_tile < j.tokens) {
+                uint8_t* ws = (uint8_t*)a.workspace;
+                const uint32_t head = j.head * group + head_in_group;
+                const uint64_t row_at = (uint64_t)tok * a.q_heads + head;
+                if (j.place == kPlaceDirect) {
+                    out = (uint8_t*)(a.out + (uint64_t)tok * a.out_token_stride + (uint64_t)head * a.out_head_stride);
+                    f = sum == 0.f ? 0.f : 1.f / sum;
+                    if (a.lse) ((float*)a.lse)[row_at] = sum == 0.f ? -INFINITY : (top * c + log2f(sum)) * 0.6931471805599453f;
+                } else {
+                    const bool home = j.place == kPlaceHome;
+                    const uint64_t at = home ? home_index(d, j.own, row_at, a.q_heads) : part_index(d, j.own, j.place, row);
+                    out = ws + (home ? w.home_o : w.part_o) + 4 * at * a.head_dim;
+                    *((float2*)(ws + (home ? w.home_ml : w.part_ml)) + at) = make_float2(top == -INFINITY ? -INFINITY : top * c, sum);
+                }
+            }
+#pragma unroll 1
+            for (int k = 0; k < (int)a.head_dim; k += 16) {
+                float o[16];
+                tmem_ld16((uint32_t*)o, t_o + k);
+                tmem_wait_ld();
+                if (!out) continue;
+                const bool half = k + 8 >= (int)a.head_dim;                       // head_dim is a multiple of 8
+                if (j.place == kPlaceDirect) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 8)
+                        if (e == 0 || !half)
+                            *(uint4*)(out + 2 * (k + e)) = make_uint4(pack2<T>(o[e] * f, o[e + 1] * f), pack2<T>(o[e + 2] * f, o[e + 3] * f),
+                                                                      pack2<T>(o[e + 4] * f, o[e + 5] * f), pack2<T>(o[e + 6] * f, o[e + 7] * f));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        if (e < 8 || !half) *(float4*)(out + 4 * (k + e)) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+            }
+            fence_before();
         }
     }
     fence_before();
@@ -714,6 +740,8 @@ cudaError_t launch_prefix_attention_tiles(const tsw_prefix_attention_args& a, co
     p.a = a;
     p.d = Deal{a.batch, a.max_q, a.cache.page_size, a.kv_heads, a.prefix_len, a.causal, w};
     p.status = status;
+    p.own_shift = __builtin_ctz(a.cache.page_size);
+    p.prefix_shift = a.prefix_len ? __builtin_ctz(a.prefix.page_size) : 0;
     cudaError_t err = encode_pages(&p.k_own, a, a.cache, false);
     if (err == cudaSuccess) err = encode_pages(&p.v_own, a, a.cache, true);
     if (err == cudaSuccess) err = encode_queries(&p.q_own, a, w.group, w.own_box_tokens);

@@ -267,7 +267,6 @@ struct Cursor {
 
 // The order in which a CTA's key tiles pass through the rings: first the prefix list, then the own list.  A list that
 // is dealt in pairs is on the first cursor alone; otherwise the two streams' tiles take turns while both have some.
-// The warps that load K, V and Q and the one that issues the products each walk it on their own.
 struct Walk {
     Cursor c0, c1;
     Job j0, j1;
@@ -312,8 +311,47 @@ struct Walk {
     }
 };
 
+// What the warps are told.  A unit is one key tile for one stream; the two units of a pair's tile share one load.
+struct alignas(16) Unit {
+    uint32_t flags;          // kUnit*, keys of the tile from bit 8, key head from bit 16
+    int tile, b, pad;
+};
+enum { kUnitStream = 1, kUnitLoad = 2, kUnitRelease = 4, kUnitFirst = 8, kUnitOwn = 16, kUnitEnd = 32 };
+TSW_HD int unit_keys(uint32_t flags) { return (flags >> 8 & 0xff) + 1; }
+TSW_HD int unit_head(uint32_t flags) { return flags >> 16; }
+// A stream's share of a job: its rows, how many tiles, and where the result goes.
+struct alignas(16) RowJob {
+    int head, tok, tokens, tiles;    // tiles = 0: no more
+    int keys, limit;                 // from the range's first key: row of token t sees keys below min(keys, limit + t)
+    int own, place;                  // place >= 0: partial result of a range that continues an item
+};
+enum { kPlaceDirect = -2, kPlaceHome = -1 };
+
 // End of what stream s sees of the job's keys (pairs: each row tile its own).
 TSW_HD int seen_by(const Job& j, bool pair, int s) { return pair && s ? j.kt_b : j.kt_a; }
+TSW_HD Unit make_unit(const Job& j, int tile, int s, bool use0, bool use1) {
+    Unit u;
+    const int keys = imin(kTile, j.keys - tile * kTile);
+    u.flags = (s ? kUnitStream : 0) | (s && use0 ? 0 : kUnitLoad) | (!s && use1 ? 0 : kUnitRelease) | (tile == j.kt0 ? kUnitFirst : 0) |
+              (j.own ? kUnitOwn : 0) | (uint32_t)(keys - 1) << 8 | (uint32_t)j.head << 16;
+    u.tile = tile;
+    u.b = j.b;
+    u.pad = 0;
+    return u;
+}
+TSW_HD RowJob make_row_job(const Deal& d, const Job& j, bool pair, int s, uint32_t cta) {
+    RowJob r;
+    const int seen = seen_by(j, pair, s), end = imin(j.kt1, seen);
+    r.head = j.head;
+    r.tok = j.tok + (pair && s ? (int)d.w.tile_tokens : 0);
+    r.tokens = pair && s ? j.n_b : j.n_a;
+    r.tiles = end - j.kt0;
+    r.keys = j.keys - j.kt0 * kTile;
+    r.limit = j.limit + 1 - j.kt0 * kTile;
+    r.own = j.own;
+    r.place = j.kt0 ? (int)part_place(pair, range_index(d, pair, cta, s), s) : !d.prefix_len && end == seen ? (int)kPlaceDirect : (int)kPlaceHome;
+    return r;
+}
 
 // Where the partial results of one row lie: of each list the ranges first .. last, its half of a pair and its
 // token's place in the row tile.  `before`: own tiles of the row's sequence in front of its item (one head).
