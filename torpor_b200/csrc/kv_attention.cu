@@ -89,6 +89,15 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uin
     return __all_sync(~0u, ok);
 }
 
+// One lane of a converged warp, chosen in a way that leaves the code under it uniform: operands of the tensor and
+// copy units are uniform registers.
+__device__ __forceinline__ bool elect() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(~0u, x, 0); }
+
 __device__ __forceinline__ void load_box4(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
@@ -183,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
     __shared__ uint32_t s_tmem, s_scan[kThreads / 32];
     __shared__ uint32_t s_gave_up;
     volatile uint32_t* gave_up = &s_gave_up;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
     const tsw_prefix_attention_args& a = p.a;
     const Deal& d = p.d;
     const AttentionLayout& w = d.w;
@@ -268,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
     __syncthreads();
     fence_after();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = uniform(s_tmem);
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
@@ -366,9 +375,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
             for (uint32_t n = 0; ok; ++n) {
                 ok = wait(bar + B::unit_full + 8 * (n % kUnits), n / kUnits & 1, gave_up);
                 if (!ok) break;
-                const uint32_t flags = s_units[n % kUnits].flags;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar + B::unit_empty + 8 * (n % kUnits));
+                const uint32_t flags = uniform(s_units[n % kUnits].flags);
+                if (elect()) mbar_arrive(bar + B::unit_empty + 8 * (n % kUnits));
                 const bool same = !((flags ^ old) & kUnitStream);
 #pragma unroll 1
                 for (int step = 0; step < 2 && ok; ++step) {
@@ -395,12 +403,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
                         if (!ok) break;
                         n_p ^= 1u << s;
                         fence_after();
-                        if (lane == 0) {
-                            const uint32_t base = tmem + s * 256, v_lo = desc_lo(v, kHalfBytes);
-                            mma_ts(base + 128, base, desc(v_lo), kDescO, !(old & kUnitFirst));
+                        const uint32_t base = tmem + s * 256, v_lo = desc_lo(v, kHalfBytes);
+                        const bool more = !(old & kUnitFirst);
+                        if (elect()) {
+                            if (keys == kTile) {
 #pragma unroll
-                            for (int k = 1; k < kTile / 16; ++k)
-                                if (k < steps) mma_ts(base + 128, base + k * 8, desc(v_lo + (k * 2048 >> 4)), kDescO, true);
+                                for (int k = 0; k < kTile / 16; ++k) mma_ts(base + 128, base + k * 8, desc(v_lo + (k * 2048 >> 4)), kDescO, k > 0 || more);
+                            } else {
+#pragma unroll 1
+                                for (int k = 0; k < steps; ++k) mma_ts(base + 128, base + k * 8, desc(v_lo + (k * 2048 >> 4)), kDescO, k > 0 || more);
+                            }
                             mma_commit(bar + B::o_full + 8 * s);
                             if (old & kUnitRelease) mma_commit(bar + B::v_empty + 8 * old_v_slot);
                         }
@@ -415,8 +427,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
                         }
                         if (!ok) break;
                         fence_after();
-                        if (lane == 0) {
-                            const uint32_t q_lo = desc_lo(q_at + s * S::kTileBytes, 16), k_lo = desc_lo(k_at + k_slot * S::kTileBytes, 16);
+                        const uint32_t q_lo = desc_lo(q_at + s * S::kTileBytes, 16), k_lo = desc_lo(k_at + k_slot * S::kTileBytes, 16);
+                        if (elect()) {
 #pragma unroll
                             for (int i = 0; i < DP / 16; ++i) {
                                 const uint32_t off = ((i / 4) * kHalfBytes + (i % 4) * 32) >> 4;
@@ -572,26 +584,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
                     *((float2*)(ws + (home ? w.home_ml : w.part_ml)) + at) = make_float2(top == -INFINITY ? -INFINITY : top * c, sum);
                 }
             }
-#pragma unroll 1
-            for (int k = 0; k < (int)a.head_dim; k += 16) {
-                float o[16];
-                tmem_ld16((uint32_t*)o, t_o + k);
-                tmem_wait_ld();
-                if (!out) continue;
-                const bool half = k + 8 >= (int)a.head_dim;                       // head_dim is a multiple of 8
-                if (j.place == kPlaceDirect) {
+            float o[DP];
 #pragma unroll
-                    for (int e = 0; e < 16; e += 8)
-                        if (e == 0 || !half)
-                            *(uint4*)(out + 2 * (k + e)) = make_uint4(pack2<T>(o[e] * f, o[e + 1] * f), pack2<T>(o[e + 2] * f, o[e + 3] * f),
-                                                                      pack2<T>(o[e + 4] * f, o[e + 5] * f), pack2<T>(o[e + 6] * f, o[e + 7] * f));
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        if (e < 8 || !half) *(float4*)(out + 4 * (k + e)) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                }
-            }
+            for (int k = 0; k < DP; k += 32) tmem_ld32((uint32_t*)o + k, t_o + k);
+            tmem_wait_ld();
             fence_before();
+            if (!out) continue;
+            if (j.place == kPlaceDirect) {
+#pragma unroll
+                for (int e = 0; e < DP; e += 8)
+                    if (e < (int)a.head_dim)                                      // a multiple of 8
+                        *(uint4*)(out + 2 * e) = make_uint4(pack2<T>(o[e] * f, o[e + 1] * f), pack2<T>(o[e + 2] * f, o[e + 3] * f),
+                                                            pack2<T>(o[e + 4] * f, o[e + 5] * f), pack2<T>(o[e + 6] * f, o[e + 7] * f));
+            } else {
+#pragma unroll
+                for (int e = 0; e < DP; e += 4)
+                    if (e < (int)a.head_dim) *(float4*)(out + 4 * e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
         }
     }
     fence_before();
