@@ -1,6 +1,5 @@
 // The dealing of the attention kernel's work (csrc/kv_dealing.hpp), run on the host for random batches: every
-// (row tile, head, key tile) is taken exactly once; loads, releases and first tiles are
-// marked where they belong; what the joining kernel reads of a row is exactly what was written for it; every index
+// (row tile, head, key tile) is taken exactly once, in whole units; what the joining kernel reads of a row is exactly what was written for it; every index
 // stays inside its table or the workspace.
 //   kv_dealing_probe SEED CASES
 #include <cstdio>
@@ -103,7 +102,7 @@ int main(int argc, char** argv) {
                 const Range g = range_at(d, w.own_pair, total, cta, s);
                 const uint32_t x = g.x, left = g.end - g.x;
                 // the kernel's threads look through pieces of the sequences; one of them holds x
-                const int each = (batch + 383) / 384;
+                const int each = (batch + 415) / 416;
                 int found = 0;
                 for (int lo = 0; left && lo < batch; lo += each) {
                     const int hi = std::min(batch, lo + each);
@@ -116,28 +115,30 @@ int main(int argc, char** argv) {
             // what the scheduling warp tells the others: units and rows' jobs
             Walk walk(d, pro);
             Job j;
-            int tile, left[2] = {0, 0}, loaded = 0;
+            int tile, left[2] = {0, 0};
             bool use[2];
             while (walk.next(d, pro, j, tile, use[0], use[1])) {
                 ++tiles_seen;
                 REQUIRE(use[0] || use[1]);
+                REQUIRE(walk.pair || !(use[0] && use[1]));
                 REQUIRE(tile >= j.kt0 && tile < j.kt1 && tile * kTile < j.keys && j.head < 65536);
                 const tsw_kv_pages& pg = j.own ? a.cache : a.prefix;
+                const Load l = make_load(j, tile, walk.pair, use[1]);
+                const int n = load_keys(l.flags), box = std::min((int)pg.page_size, kTile), first = tile * kTile / (int)pg.page_size;
+                REQUIRE(n == std::min(kTile, j.keys - tile * kTile) && n >= 1 && load_head(l.flags) == j.head && l.b == j.b && l.tile == tile);
+                REQUIRE(first + (n + box - 1) / box - 1 < (j.own ? width : ((int)a.prefix_len + page_size - 1) / page_size));
+                REQUIRE(((l.flags & kLoadOwn) != 0) == (j.own == 1) && !(l.flags & kLoadEnd) && ((l.flags & kLoadPair) != 0) == walk.pair);
+                REQUIRE(walk.pair || ((l.flags & kLoadSecond) != 0) == use[1]);
                 for (int s = 0; s < 2; ++s) {
+                    const uint32_t u = make_take(j, tile, use[s], walk.pair, tile % 5, tile % 6);
+                    REQUIRE(((u & kTakeSkip) != 0) == !use[s] && ((u & kTakePair) != 0) == walk.pair && !(u & kTakeEnd) && take_keys(u) == n &&
+                            k_slot(u) == (uint32_t)tile % 5 && v_slot(u) == (uint32_t)tile % 6);
                     if (!use[s]) continue;
-                    const Unit u = make_unit(j, tile, s, use[0], use[1]);
-                    const int n = unit_keys(u.flags), box = std::min((int)pg.page_size, kTile), first = tile * kTile / (int)pg.page_size;
-                    REQUIRE(n == std::min(kTile, j.keys - tile * kTile) && n >= 1 && unit_head(u.flags) == j.head);
-                    REQUIRE(first + (n + box - 1) / box - 1 < (j.own ? width : ((int)a.prefix_len + page_size - 1) / page_size));
-                    REQUIRE(((u.flags & kUnitStream) != 0) == (s == 1) && ((u.flags & kUnitOwn) != 0) == (j.own == 1));
-                    loaded += (u.flags & kUnitLoad) ? 1 : 0;
-                    REQUIRE(loaded == 1);                              // one load in front of the tile's units
-                    loaded -= (u.flags & kUnitRelease) ? 1 : 0;
                     const RowJob r = make_row_job(d, j, walk.pair, s, cta);
-                    REQUIRE(((u.flags & kUnitFirst) != 0) == (left[s] == 0));
-                    if (u.flags & kUnitFirst) {
-                        left[s] = r.tiles;
-                        REQUIRE(r.tiles >= 1 && r.tokens >= 1 && r.tokens <= (int)w.tile_tokens && r.tok >= 0 && r.tok + r.tokens <= tokens);
+                    REQUIRE(((u & kTakeFirst) != 0) == (left[s] == 0));
+                    if (u & kTakeFirst) {
+                        left[s] = r.units;
+                        REQUIRE(r.units >= 1 && r.tokens >= 1 && r.tokens <= (int)w.tile_tokens && r.tok >= 0 && r.tok + r.tokens <= tokens);
                         for (int i = 0; i < r.tokens * group; ++i) {
                             const uint64_t row = (uint64_t)(r.tok + i / group) * a.q_heads + r.head * group + i % group;
                             if (r.place == kPlaceDirect) ++direct[row];
@@ -150,10 +151,10 @@ int main(int argc, char** argv) {
                             }
                         }
                     }
-                    --left[s];
+                    left[s] -= units_of(n);
+                    REQUIRE(left[s] >= 0);
                     REQUIRE(done.insert({j.own, r.tok, j.head, tile}).second);
                 }
-                REQUIRE(loaded == 0);
             }
             REQUIRE(left[0] == 0 && left[1] == 0);
         }

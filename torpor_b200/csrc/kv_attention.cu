@@ -25,6 +25,7 @@
 
 #include <atomic>
 #include <cstring>
+#include <type_traits>
 
 #include <cuda.h>
 
@@ -32,8 +33,9 @@ namespace tsw {
 
 namespace {
 
-constexpr int kThreads = 384;                 // two warpgroups of rows; warps for K, V, the products, Q
-constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr int kThreads = 416;                 // two warpgroups of rows; warps for keys, values, each stream's products, scheduling
+constexpr unsigned long long kWaitNs = 2000000000ull, kDrainNs = 5000000ull;
+constexpr int kByHand = 0;                    // of 8 pairs of exponentials
 constexpr float kGrow = 8.f;                  // log2 of the growth of the maximum that is let pass
 
 template <int DP> struct Shape {
@@ -70,6 +72,12 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {      // does not wait
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ unsigned long long now() {
     unsigned long long t;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
@@ -87,6 +95,17 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uin
         if (!ok && now() - t0 > kWaitNs) *gave_up = 1;
     } while (!__all_sync(~0u, ok) && !__any_sync(~0u, *gave_up));
     return __all_sync(~0u, ok);
+}
+
+__device__ __forceinline__ bool wait_alone(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {      // one thread's wait
+    if (mbar_try(bar, parity)) return true;
+    const unsigned long long t0 = now();
+#pragma unroll 1
+    while (!mbar_try(bar, parity)) {
+        if (now() - t0 > kWaitNs) *gave_up = 1;
+        if (*gave_up) return false;
+    }
+    return true;
 }
 
 // One lane of a converged warp, chosen in a way that leaves the code under it uniform: operands of the tensor and
@@ -143,6 +162,50 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two floats to an instruction.
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 split(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x of two numbers without the special function unit, for finite x <= 8 (or below: 2^-125 at least comes back).  x is
+// split into the nearest integer, which goes into the exponent, and a rest in [-1/2, 1/2], where a polynomial of
+// degree 5 fitted to the least relative error (Remez exchange) is within 2^-23 of 2^rest.
+__device__ __forceinline__ float2 exp2_two(float2 x) {
+    constexpr float kRound = 12582912.f;                 // 1.5 * 2^23: adding it rounds to an integer, kept in the low bits
+    const uint64_t v = two(fmaxf(x.x, -125.f), fmaxf(x.y, -125.f));
+    const uint64_t t = add2(v, two(kRound, kRound));
+    const uint64_t f = fma2(add2(t, two(-kRound, -kRound)), two(-1.f, -1.f), v);
+    uint64_t p = two(1.3276472454890609e-3f, 1.3276472454890609e-3f);
+    p = fma2(p, f, two(9.675540961325169e-3f, 9.675540961325169e-3f));
+    p = fma2(p, f, two(5.550713092088699e-2f, 5.550713092088699e-2f));
+    p = fma2(p, f, two(0.24022120237350464f, 0.24022120237350464f));
+    p = fma2(p, f, two(0.6931469440460205f, 0.6931469440460205f));
+    p = fma2(p, f, two(1.0000001192092896f, 1.0000001192092896f));
+    const float2 n = split(t), m = split(p);
+    return make_float2(__uint_as_float((__float_as_uint(n.x) << 23) + __float_as_uint(m.x)),
+                       __uint_as_float((__float_as_uint(n.y) << 23) + __float_as_uint(m.y)));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
     uint32_t r;
@@ -167,15 +230,21 @@ __device__ __forceinline__ uint64_t desc(uint32_t lo) {
     return r;
 }
 
-constexpr int kUnits = 16;                    // units on their way from the scheduling warp to the others
-constexpr int kJobs = 4;                      // rows' jobs on their way, per stream
+// What the scheduling warp has told the others and they have not yet taken up: loads; takes and rows' jobs of a stream.
+constexpr int kLoads = 8, kTakes = 4, kJobs = 4;
 
-// mbarriers: byte offsets into the array in shared memory
+// Warps behind the rows' eight.
+enum { kWarpK = 8, kWarpV, kWarpSchedule, kWarpProducts };      // kWarpProducts + stream
+
+// mbarriers: byte offsets into the array in shared memory.  Pairs and rings of a stream lie together.
 template <int kK, int kV> struct Bars {
-    static constexpr int k_full = 0, k_empty = k_full + 8 * kK, v_full = k_empty + 8 * kK, v_empty = v_full + 8 * kV, q_full = v_empty + 8 * kV,
-                         s_full = q_full + 16, o_full = s_full + 16, unit_full = o_full + 16, job_full = unit_full + 8 * kUnits,
-                         ones = (job_full + 16 * kJobs) / 8,                          // up to here one arrival completes a phase
-                         unit_empty = 8 * ones, p_full = unit_empty + 8 * kUnits, job_empty = p_full + 16, bytes = job_empty + 16 * kJobs;
+    static constexpr int k_full = 0, v_full = k_full + 16 * kK, q_full = v_full + 16 * kV, o_full = q_full + 16, s_full = o_full + 32,
+                         load_full = s_full + 32, take_full = load_full + 8 * kLoads, take_empty = take_full + 16 * kTakes,
+                         job_full = take_empty + 16 * kTakes,
+                         ones = (job_full + 16 * kJobs) / 8,                         // up to here one arrival ends a phase
+                         k_empty = 8 * ones, v_empty = k_empty + 8 * kK, load_empty = v_empty + 8 * kV,
+                         p_full = load_empty + 8 * kLoads,                           // up to here two, from here four
+                         job_empty = p_full + 32, bytes = job_empty + 16 * kJobs;
 };
 
 template <typename T, int DP>
@@ -186,10 +255,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
     constexpr uint32_t kHalfBytes = kTile * 128;
     extern __shared__ uint8_t s_raw[];
     __shared__ __align__(8) uint64_t s_bars[B::bytes / 8];
-    __shared__ Unit s_units[kUnits];
+    __shared__ Load s_loads[kLoads];
+    __shared__ uint32_t s_takes[2][kTakes];
     __shared__ RowJob s_jobs[2][kJobs];
+    __shared__ uint32_t s_last[2][2 * kJobs];      // slot of the values of a job's last tile: read up to kJobs jobs later
     __shared__ Prologue s_pro;
-    __shared__ uint32_t s_tmem, s_scan[kThreads / 32];
+    __shared__ uint32_t s_tmem, s_scan[(kThreads + 31) / 32];
     __shared__ uint32_t s_gave_up;
     volatile uint32_t* gave_up = &s_gave_up;
     const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
@@ -209,16 +280,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
         wrong |= read_rows(a.batch, b, a.max_q, a.cache.page_size, r);
         mine += sequence_tiles(d, r);
     }
-    if (warp == 10) {
+    if (warp == kWarpSchedule) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    if (warp == 9) {
+    if (warp == kWarpV) {
         for (int i = lane; i < B::bytes / 8; i += 32)
-            mbar_init(bar + 8 * i, i < B::ones ? 1 : i < B::p_full / 8 ? 3 : 4);
+            mbar_init(bar + 8 * i, i < B::ones ? 1 : i < B::p_full / 8 ? 2 : 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8 && lane < 6) {
+    if (warp == kWarpK && lane < 6) {
         const CUtensorMap* map = &p.q_prefix + lane;
         asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
     }
@@ -238,11 +309,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
     __syncthreads();
     uint32_t total = 0;
 #pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) {
+    for (int i = 0; i < (kThreads + 31) / 32; ++i) {
         if (i == warp) before += total;
         total += s_scan[i];
     }
-    if (warp == 11) {
+    if (warp == kWarpSchedule) {
         int tok0, tok1;
         const uint32_t rts = prefix_rows(d, tok0, tok1), prefix_total = a.kv_heads * rts * w.prefix_tiles;
         if (lane < 2) s_pro.prefix[lane] = range_at(d, w.prefix_pair, prefix_total, blockIdx.x, lane);
@@ -279,184 +350,199 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = uniform(s_tmem);
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        if (warp == 11) {
-            // ------------------------------------------------------------ scheduling
+    if (warp == kWarpSchedule) {
+        // ---------------------------------------------------------------- scheduling, by one thread
+        if (elect()) {
             Walk walk(d, s_pro);
             Job j;
             int tile;
-            uint32_t n = 0, jobs[2] = {0, 0};
-            bool use[2], ok = true;
+            uint32_t n = 0, takes[2] = {0, 0}, jobs[2] = {0, 0};
+            Ring k{0, 0}, v{0, 0};
+            bool use[2], ok = true, more = true;
 #pragma unroll 1
-            while (ok) {
-                const bool more = walk.next(d, s_pro, j, tile, use[0], use[1]);
-                if (!more) use[0] = use[1] = true;
-#pragma unroll 1
-                for (int s = 0; s < 2 && ok; ++s) {
-                    if (s ? !use[1] : !use[0]) continue;
-                    if (!more || tile == j.kt0) {                     // also tells both streams' rows of the end
-                        const uint32_t i = s ? jobs[1]++ : jobs[0]++, at = s * kJobs + i % kJobs;
-                        ok = wait(bar + B::job_empty + 8 * at, (i / kJobs & 1) ^ 1, gave_up);
-                        if (!ok) break;
-                        if (lane == 0) {
+            while (ok && more) {
+                more = walk.next(d, s_pro, j, tile, use[0], use[1]);
+                if (!more) use[0] = use[1] = true;                    // the end is told to everyone
+                ok = wait_alone(bar + B::load_empty + 8 * (n % kLoads), (n / kLoads & 1) ^ 1, gave_up);
+                if (!ok) break;
+                s_loads[n % kLoads] = more ? make_load(j, tile, walk.pair, use[1]) : Load{kLoadEnd, 0, 0, 0};
+                mbar_arrive(bar + B::load_full + 8 * (n % kLoads));
+                ++n;
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    if (!ok || (!use[s] && !walk.pair)) continue;
+                    if (use[s]) {
+                        if (!more || tile == j.kt0) {
+                            const uint32_t i = jobs[s]++, at = s * kJobs + i % kJobs;
+                            ok = wait_alone(bar + B::job_empty + 8 * at, (i / kJobs & 1) ^ 1, gave_up);
+                            if (!ok) continue;
                             RowJob r = {};
                             if (more) r = make_row_job(d, j, walk.pair, s, blockIdx.x);
                             s_jobs[s][i % kJobs] = r;
                             mbar_arrive(bar + B::job_full + 8 * at);
                         }
-                        if (!more && s == 0) continue;
+                        if (more && tile + 1 == min(j.kt1, seen_by(j, walk.pair, s))) s_last[s][(jobs[s] - 1) % (2 * kJobs)] = v.slot;
                     }
-                    ok = wait(bar + B::unit_empty + 8 * (n % kUnits), (n / kUnits & 1) ^ 1, gave_up);
-                    if (!ok) break;
-                    if (lane == 0) {
-                        s_units[n % kUnits] = more ? make_unit(j, tile, s, use[0], use[1]) : Unit{kUnitEnd, 0, 0, 0};
-                        mbar_arrive(bar + B::unit_full + 8 * (n % kUnits));
-                    }
-                    ++n;
+                    const uint32_t i = takes[s]++, at = s * kTakes + i % kTakes;
+                    ok = wait_alone(bar + B::take_empty + 8 * at, (i / kTakes & 1) ^ 1, gave_up);
+                    if (!ok) continue;
+                    s_takes[s][i % kTakes] = more ? make_take(j, tile, use[s], walk.pair, k.slot, v.slot) : (uint32_t)kTakeEnd;
+                    mbar_arrive(bar + B::take_full + 8 * at);
                 }
-                if (!more) break;
-            }
-        } else if (warp < 10) {
-            // ------------------------------------------------------------ keys (8) and values (9)
-            const bool is_v = warp == 9;
-            const int stages = is_v ? S::kV : S::kK;
-            const uint32_t at = is_v ? v_at : k_at, full = bar + (is_v ? B::v_full : B::k_full), empty = bar + (is_v ? B::v_empty : B::k_empty);
-            int slot = 0;
-            uint32_t phase = 0, issued = 0;
-#pragma unroll 1
-            for (uint32_t n = 0;; ++n) {
-                if (!wait(bar + B::unit_full + 8 * (n % kUnits), n / kUnits & 1, gave_up)) break;
-                const Unit u = s_units[n % kUnits];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar + B::unit_empty + 8 * (n % kUnits));
-                if (u.flags & kUnitEnd) break;
-                if (!(u.flags & kUnitLoad)) continue;
-                const bool own = u.flags & kUnitOwn;
-                const tsw_kv_pages& pg = own ? a.cache : a.prefix;
-                const CUtensorMap* map = own ? (is_v ? &p.v_own : &p.k_own) : (is_v ? &p.v_prefix : &p.k_prefix);
-                const int shift = own ? p.own_shift : p.prefix_shift, box = min(1 << shift, kTile);
-                const int boxes = (unit_keys(u.flags) + box - 1) / box, first = u.tile * kTile >> shift, in_page = u.tile * kTile & ((1 << shift) - 1);
-                const int* table = (own ? (const int*)a.batch.page_table + (uint64_t)u.b * a.batch.table_stride : (const int*)a.prefix_table) + first;
-                int page = lane < boxes ? table[lane] : 0;                // before the wait: its latency passes under it
-                if (!wait(empty + 8 * slot, phase ^ 1, gave_up)) break;
-                if (lane == 0) mbar_expect(full + 8 * slot, boxes * box * 128 * kHalves);
-                __syncwarp();
-#pragma unroll 1
-                for (int i = lane; i < boxes; i += 32) {
-                    if (i >= 32) page = table[i];
-                    // a number outside the cache is recorded; the copy unit fills such a box with zeros
-                    if ((uint32_t)page >= pg.pages) { atomicOr(p.status, TSW_KV_BAD_PAGE); page = pg.pages; }
-                    const uint32_t dst = at + slot * S::kTileBytes + i * box * 128;
-#pragma unroll
-                    for (int h = 0; h < kHalves; ++h)
-                        load_box4(dst + h * kHalfBytes, map, h * 64, in_page, unit_head(u.flags), page, full + 8 * slot);
-                }
-                ++issued;
-                if (++slot == stages) { slot = 0; phase ^= 1; }
-            }
-            if (*gave_up)        // copies in flight land before the CTA ends
-                for (int i = 0; i < stages && i < (int)issued; ++i) {
-                    const unsigned long long t0 = now();
-                    while (!mbar_try(full + 8 * i, i < slot ? phase : phase ^ 1) && now() - t0 < kWaitNs / 8) {}
-                }
-        } else {
-            // ------------------------------------------------------------ products
-            // Order: S of a unit, then the O product of the unit before it, whose exponentials ran meanwhile.  When both
-            // are one stream's, O goes first: S would overwrite the weights.
-            constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u << 7 | 1u << 10;
-            constexpr uint32_t kDescS = 1u << 4 | kType | (kTile / 8) << 17 | (kTile / 16) << 24;
-            constexpr uint32_t kDescO = 1u << 4 | kType | 1u << 16 | (DP / 8) << 17 | (kTile / 16) << 24;
-            uint32_t n_q = 0, n_p = 0;                    // phases of both streams, bit s
-            int k_slot = 0, v_slot = 0, old_v_slot = 0;
-            uint32_t k_phase = 0, v_phase = 0, old_v_phase = 0, old = kUnitEnd;
-            bool ok = true;
-#pragma unroll 1
-            for (uint32_t n = 0; ok; ++n) {
-                ok = wait(bar + B::unit_full + 8 * (n % kUnits), n / kUnits & 1, gave_up);
-                if (!ok) break;
-                const uint32_t flags = uniform(s_units[n % kUnits].flags);
-                if (elect()) mbar_arrive(bar + B::unit_empty + 8 * (n % kUnits));
-                const bool same = !((flags ^ old) & kUnitStream);
-#pragma unroll 1
-                for (int step = 0; step < 2 && ok; ++step) {
-                    if ((step == 0) == same) {
-                        if (old & kUnitEnd) continue;
-                        const int s = old & kUnitStream, keys = unit_keys(old), steps = (keys + 15) / 16;
-                        const uint32_t v = v_at + old_v_slot * S::kTileBytes;
-                        if (old & kUnitLoad) {
-                            ok = wait(bar + B::v_full + 8 * old_v_slot, old_v_phase, gave_up);
-                            if (ok && (keys & 15)) {
-                                // Rows behind the last key hold whatever their page holds, and a weight of zero
-                                // does not silence an infinity: clear what the last step would read.
-                                const int rows = steps * 16 - keys;
-#pragma unroll 1
-                                for (int i = lane; i < rows * 8 * kHalves; i += 32) {
-                                    const uint32_t to = v + (i / (rows * 8)) * kHalfBytes + (keys + (i / 8) % rows) * 128 + (i % 8) * 16;
-                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
-                                }
-                                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                                __syncwarp();
-                            }
-                        }
-                        ok = ok && wait(bar + B::p_full + 8 * s, n_p >> s & 1, gave_up);
-                        if (!ok) break;
-                        n_p ^= 1u << s;
-                        fence_after();
-                        const uint32_t base = tmem + s * 256, v_lo = desc_lo(v, kHalfBytes);
-                        const bool more = !(old & kUnitFirst);
-                        if (elect()) {
-                            if (keys == kTile) {
-#pragma unroll
-                                for (int k = 0; k < kTile / 16; ++k) mma_ts(base + 128, base + k * 8, desc(v_lo + (k * 2048 >> 4)), kDescO, k > 0 || more);
-                            } else {
-#pragma unroll 1
-                                for (int k = 0; k < steps; ++k) mma_ts(base + 128, base + k * 8, desc(v_lo + (k * 2048 >> 4)), kDescO, k > 0 || more);
-                            }
-                            mma_commit(bar + B::o_full + 8 * s);
-                            if (old & kUnitRelease) mma_commit(bar + B::v_empty + 8 * old_v_slot);
-                        }
-                        __syncwarp();
-                    } else {
-                        if (flags & kUnitEnd) continue;
-                        const int s = flags & kUnitStream;
-                        if (flags & kUnitLoad) ok = wait(bar + B::k_full + 8 * k_slot, k_phase, gave_up);
-                        if (ok && (flags & kUnitFirst)) {
-                            ok = wait(bar + B::q_full + 8 * s, n_q >> s & 1, gave_up);
-                            n_q ^= 1u << s;
-                        }
-                        if (!ok) break;
-                        fence_after();
-                        const uint32_t q_lo = desc_lo(q_at + s * S::kTileBytes, 16), k_lo = desc_lo(k_at + k_slot * S::kTileBytes, 16);
-                        if (elect()) {
-#pragma unroll
-                            for (int i = 0; i < DP / 16; ++i) {
-                                const uint32_t off = ((i / 4) * kHalfBytes + (i % 4) * 32) >> 4;
-                                mma_ss(tmem + s * 256, desc(q_lo + off), desc(k_lo + off), kDescS, i > 0);
-                            }
-                            mma_commit(bar + B::s_full + 8 * s);
-                            if (flags & kUnitRelease) mma_commit(bar + B::k_empty + 8 * k_slot);
-                        }
-                        __syncwarp();
-                    }
-                }
-                if (flags & kUnitEnd) break;
-                old = flags;
-                old_v_slot = v_slot;
-                old_v_phase = v_phase;
-                if (flags & kUnitRelease) {
-                    if (++k_slot == S::kK) { k_slot = 0; k_phase ^= 1; }
-                    if (++v_slot == S::kV) { v_slot = 0; v_phase ^= 1; }
-                }
+                k.step(S::kK);
+                v.step(S::kV);
             }
         }
+        __syncwarp();
+    } else if (warp == kWarpK || warp == kWarpV) {
+        // ---------------------------------------------------------------- keys and values
+        const bool is_v = warp == kWarpV;
+        const uint32_t stages = is_v ? S::kV : S::kK;
+        const uint32_t at = is_v ? v_at : k_at, full = bar + (is_v ? B::v_full : B::k_full), empty = bar + (is_v ? B::v_empty : B::k_empty);
+        Ring ring{0, 0};
+#pragma unroll 1
+        for (uint32_t n = 0;; ++n) {
+            if (!wait(bar + B::load_full + 8 * (n % kLoads), n / kLoads & 1, gave_up)) break;
+            const Load u = s_loads[n % kLoads];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar + B::load_empty + 8 * (n % kLoads));
+            if (u.flags & kLoadEnd) break;
+            const bool own = u.flags & kLoadOwn;
+            const tsw_kv_pages& pg = own ? a.cache : a.prefix;
+            const CUtensorMap* map = own ? (is_v ? &p.v_own : &p.k_own) : (is_v ? &p.v_prefix : &p.k_prefix);
+            const int shift = own ? p.own_shift : p.prefix_shift, box = min(1 << shift, kTile);
+            const int boxes = (load_keys(u.flags) + box - 1) / box, first = u.tile * kTile >> shift, in_page = u.tile * kTile & ((1 << shift) - 1);
+            const int* table = (own ? (const int*)a.batch.page_table + (uint64_t)u.b * a.batch.table_stride : (const int*)a.prefix_table) + first;
+            int page = lane < boxes ? table[lane] : 0;                // before the wait: its latency passes under it
+            if (!wait(empty + 8 * ring.slot, ring.phase ^ 1, gave_up)) break;
+            // Each stream has a barrier to a slot: it takes note of every phase of the ones it waits for, so their parities
+            // are never mistaken.  Tiles of a list in pairs are on the first stream's for both.
+            const uint32_t done = full + 8 * (u.flags & kLoadSecond ? stages + ring.slot : ring.slot);
+            if (lane == 0) {
+                if (!(u.flags & kLoadPair)) mbar_arrive(empty + 8 * ring.slot);       // the other stream has nothing to do with it
+                mbar_expect(done, boxes * box * 128 * kHalves);
+            }
+            __syncwarp();
+#pragma unroll 1
+            for (int i = lane; i < boxes; i += 32) {
+                if (i >= 32) page = table[i];
+                // a number outside the cache is recorded; the copy unit fills such a box with zeros
+                if ((uint32_t)page >= pg.pages) { atomicOr(p.status, TSW_KV_BAD_PAGE); page = pg.pages; }
+                const uint32_t dst = at + ring.slot * S::kTileBytes + i * box * 128;
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h)
+                    load_box4(dst + h * kHalfBytes, map, h * 64, in_page, load_head(u.flags), page, done);
+            }
+            ring.step(stages);
+        }
+    } else if (warp >= kWarpProducts) {
+        // ---------------------------------------------------------------- products of one stream, by one thread
+        // A stream has two S buffers of half a tile's keys, taken in turn; weights go back over their S.  The S product of a
+        // unit goes out in front of the O product of the unit before it, so that there is always one S for the rows to work
+        // on; it may overwrite the weights of the unit two before, whose O product is ahead of it in the tensor pipe, which
+        // takes them in order.  Nothing waits for a next tile while an O product is held back: where it is not there yet,
+        // the O product goes first.
+        constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u << 7 | 1u << 10;
+        constexpr uint32_t kDescS = 1u << 4 | kType | (kHalf / 8) << 17 | (kTile / 16) << 24;
+        constexpr uint32_t kDescO = 1u << 4 | kType | 1u << 16 | (DP / 8) << 17 | (kTile / 16) << 24;
+        const int s = warp - kWarpProducts;
+        if (elect()) {
+            const uint32_t t_s = tmem + s * 256, t_o = t_s + 128, q_lo = desc_lo(q_at + s * S::kTileBytes, 16);
+            const uint32_t b_p = bar + B::p_full + 16 * s, b_o = bar + B::o_full + 16 * s, b_s = bar + B::s_full + 16 * s;
+            const uint32_t b_tf = bar + B::take_full + 8 * kTakes * s, b_te = bar + B::take_empty + 8 * kTakes * s;
+            uint32_t k_ph = 0, v_ph = 0, q_ph = 0;                // phases of the barriers, a bit each
+            uint32_t n = 0;                                       // units whose S product has gone out
+            uint32_t held_lo = 0, held_slot = 0;                  // the unit before, whose O product has not
+            int held_steps = 0;                                   // 0: none
+            bool held_first = false, held_last = false, held_wait = false, held_pair = false, ok = true;
+            auto see_v = [&](uint32_t slot, bool pair) {
+                const uint32_t x = (pair ? 0 : s * S::kV) + slot;
+                ok = wait_alone(bar + B::v_full + 8 * x, v_ph >> x & 1, gave_up);
+                v_ph ^= 1u << x;
+                return ok;
+            };
+            auto product_o = [&]() {
+                const uint32_t buf = (n - 1) & 1, t_p = t_s + buf * kHalf;
+                if (held_wait && !see_v(held_slot, held_pair)) return;
+                ok = wait_alone(b_p + 8 * buf, (n - 1) >> 1 & 1, gave_up);
+                if (!ok) return;
+                fence_after();
+                if (held_steps == kHalf / 16) {
+#pragma unroll
+                    for (int i = 0; i < kHalf / 16; ++i) mma_ts(t_o, t_p + i * 8, desc(held_lo + (i * 2048 >> 4)), kDescO, i > 0 || !held_first);
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < held_steps; ++i) mma_ts(t_o, t_p + i * 8, desc(held_lo + (i * 2048 >> 4)), kDescO, i > 0 || !held_first);
+                }
+                mma_commit(b_o + 8 * buf);
+                if (held_last) mma_commit(bar + B::v_empty + 8 * held_slot);
+                held_steps = 0;
+            };
+#pragma unroll 1
+            for (uint32_t t = 0;; ++t) {
+                const uint32_t at = t % kTakes, par = t / kTakes & 1;
+                if (held_steps && !mbar_test(b_tf + 8 * at, par)) product_o();
+                ok = ok && wait_alone(b_tf + 8 * at, par, gave_up);
+                if (!ok) break;
+                const uint32_t u = s_takes[s][at];
+                mbar_arrive(b_te + 8 * at);
+                const bool pair = u & kTakePair, first = u & kTakeFirst;
+                const uint32_t slot = k_slot(u), x = (pair ? 0 : s * S::kK) + slot;
+                if (held_steps && ((u & (kTakeEnd | kTakeSkip | kTakeFirst)) || !mbar_test(bar + B::k_full + 8 * x, k_ph >> x & 1))) product_o();
+                if (!ok || (u & kTakeEnd)) break;
+                ok = wait_alone(bar + B::k_full + 8 * x, k_ph >> x & 1, gave_up);
+                if (!ok) break;
+                k_ph ^= 1u << x;
+                if (u & kTakeSkip) {                              // the other row tile's alone
+                    mbar_arrive(bar + B::k_empty + 8 * slot);
+                    if (!see_v(v_slot(u), pair)) break;
+                    mbar_arrive(bar + B::v_empty + 8 * v_slot(u));
+                    continue;
+                }
+                if (first) {
+                    ok = wait_alone(bar + B::q_full + 8 * s, q_ph, gave_up);
+                    if (!ok) break;
+                    q_ph ^= 1;
+                }
+                const int keys = take_keys(u), halves = units_of(keys);
+#pragma unroll 1
+                for (int h = 0; h < halves; ++h) {
+                    const int mine = min(kHalf, keys - h * kHalf);
+                    const bool tail = mine & 15;                  // the rows will clear what lies behind: the values have to be there
+                    if (tail) {
+                        if (held_steps) product_o();
+                        if (!ok || (h == 0 && !see_v(v_slot(u), pair))) break;
+                    }
+                    const uint32_t k_lo = desc_lo(k_at + slot * S::kTileBytes + h * kHalf * 128, 16), t_x = t_s + (n & 1) * kHalf;
+                    fence_after();
+#pragma unroll
+                    for (int i = 0; i < DP / 16; ++i) {
+                        const uint32_t off = ((i / 4) * kHalfBytes + (i % 4) * 32) >> 4;
+                        mma_ss(t_x, desc(q_lo + off), desc(k_lo + off), kDescS, i > 0);
+                    }
+                    mma_commit(b_s + 8 * (n & 1));
+                    if (h + 1 == halves) mma_commit(bar + B::k_empty + 8 * slot);
+                    if (held_steps) product_o();
+                    if (!ok) break;
+                    held_lo = desc_lo(v_at + v_slot(u) * S::kTileBytes + h * kHalf * 128, kHalfBytes);
+                    held_slot = v_slot(u);
+                    held_steps = (mine + 15) / 16;
+                    held_first = first && h == 0;
+                    held_last = h + 1 == halves;
+                    held_wait = h == 0 && !tail;
+                    held_pair = pair;
+                    ++n;
+                }
+                if (!ok) break;
+            }
+        }
+        __syncwarp();
     } else {
         // ---------------------------------------------------------------- rows: one thread each
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int s = warp >> 2, row = tid & 127, group = w.group;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;                 // this warp's quarter of the tensor memory's lanes
         const uint32_t t_s = tmem + lanes + s * 256, t_o = t_s + 128;
-        const uint32_t b_s = bar + B::s_full + 8 * s, b_p = bar + B::p_full + 8 * s, b_o = bar + B::o_full + 8 * s;
+        const uint32_t b_s = bar + B::s_full + 16 * s, b_p = bar + B::p_full + 16 * s, b_o = bar + B::o_full + 16 * s;
         const uint32_t b_jf = bar + B::job_full + 8 * kJobs * s, b_je = bar + B::job_empty + 8 * kJobs * s;
         const float c = a.scale * 1.4426950408889634f;
         const int tok_in_tile = row / group, head_in_group = row - tok_in_tile * group;
@@ -464,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
         uint32_t count = 0, asked = 0;                                    // units so far; jobs whose queries are on their way
         auto load_q = [&](uint32_t i) {                                   // of job i, which has been read or seen to be there
             const RowJob& j = s_jobs[s][i % kJobs];
-            if (lane == 0 && j.tiles) {
+            if (lane == 0 && j.units) {
                 const uint32_t box = j.own ? w.own_box_tokens : w.tile_tokens, to = q_at + s * S::kTileBytes;
                 const CUtensorMap* map = j.own ? &p.q_own : &p.q_prefix;
                 mbar_expect(bar + B::q_full + 8 * s, box * group * 128 * kHalves);
@@ -482,38 +568,41 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
             const RowJob j = s_jobs[s][i % kJobs];
             __syncwarp();
             if (lane == 0) mbar_arrive(b_je + 8 * (i % kJobs));
-            if (!j.tiles) break;
+            if (!j.units) break;
             const int tok = j.tok + tok_in_tile;
+            const bool mine = tok_in_tile < j.tokens;
             const bool warp_on = (warp & 3) * 32 < j.tokens * group;
             int left = min(j.keys, max(0, j.limit + tok));                // keys this row sees from here on
             float top = -INFINITY, sum = 0.f;
 #pragma unroll 1
-            for (int tile = 0; tile < j.tiles; ++tile, ++count, left -= kTile) {
-                ok = wait(b_s, count & 1, gave_up);
+            for (int unit = 0; unit < j.units; ++unit, ++count, left -= kHalf) {
+                const uint32_t buf = count & 1, t_x = t_s + buf * kHalf;
+                ok = wait(b_s + 8 * buf, count >> 1 & 1, gave_up);
                 if (!ok) break;
                 fence_after();
                 // The job's last S is there, so its queries are done with: fetch the next job's, if it is known yet.
-                if (loads_q && tile == j.tiles - 1 && __all_sync(~0u, mbar_try(b_jf + 8 * ((i + 1) % kJobs), (i + 1) / kJobs & 1))) load_q(i + 1);
+                if (loads_q && unit == j.units - 1 && __all_sync(~0u, mbar_try(b_jf + 8 * ((i + 1) % kJobs), (i + 1) / kJobs & 1))) load_q(i + 1);
                 if (warp_on) {
-                    float x[kTile];
+                    float x[kHalf];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tmem_ld32((uint32_t*)x + 32 * k, t_s + 32 * k);
+                    for (int k = 0; k < kHalf; k += 32) tmem_ld32((uint32_t*)x + k, t_x + k);
                     tmem_wait_ld();
-                    if (__any_sync(~0u, left < kTile)) {
+                    if (__any_sync(~0u, left < kHalf)) {
 #pragma unroll
-                        for (int k = 0; k < kTile; ++k)
+                        for (int k = 0; k < kHalf; ++k)
                             if (k >= left) x[k] = -INFINITY;
                     }
                     float m0 = x[0], m1 = x[1], m2 = x[2], m3 = x[3];
 #pragma unroll
-                    for (int k = 4; k < kTile; k += 4) {
-                        m0 = fmaxf(m0, x[k]);
-                        m1 = fmaxf(m1, x[k + 1]);
-                        m2 = fmaxf(m2, x[k + 2]);
-                        m3 = fmaxf(m3, x[k + 3]);
+                    for (int k = 4; k < kHalf - 4; k += 8) {
+                        m0 = max3(m0, x[k], x[k + 4]);
+                        m1 = max3(m1, x[k + 1], x[k + 5]);
+                        m2 = max3(m2, x[k + 2], x[k + 6]);
+                        m3 = max3(m3, x[k + 3], x[k + 7]);
                     }
-                    const float here = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-                    if (tile == 0) {
+                    m0 = max3(m0, x[kHalf - 4], x[kHalf - 3]);
+                    const float here = max3(fmaxf(m0, m1), fmaxf(m2, m3), fmaxf(x[kHalf - 2], x[kHalf - 1]));
+                    if (unit == 0) {
                         top = here;
                     } else {
                         const bool grow = (here - top) * c > kGrow;              // also from -inf; never between two of them
@@ -521,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
                             const float f = grow ? exp2_fast((top - here) * c) : 1.f;
                             if (grow) top = here;
                             sum *= f;
-                            ok = wait(b_o, (count - 1) & 1, gave_up);
+                            ok = wait(b_o + 8 * ((count - 1) & 1), (count - 1) >> 1 & 1, gave_up);
                             if (!ok) break;
                             fence_after();
 #pragma unroll 1
@@ -536,40 +625,65 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
                         }
                     }
                     const float base = top == -INFINITY ? 0.f : top * c;
-                    float p0 = 0.f, p1 = 0.f, p2 = 0.f, p3 = 0.f;
+                    const uint64_t c2 = two(c, c), base2 = two(-base, -base);
+                    uint64_t s0 = 0, s1 = 0;
+                    // Two warps of a scheduler share a special function unit that takes 8 cycles an instruction: 1024 cycles for
+                    // their 64 columns each, against 512 of products.  Where nothing is masked and all scores are finite,
+                    // kByHand of 8 pairs are formed by multiplications instead.
+                    const bool plain = __all_sync(~0u, !mine || (left >= kHalf && fabsf(here) < INFINITY));
+                    auto weights = [&](auto by_hand) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        uint32_t packed[16];
+                        for (int k = 0; k < kHalf / 32; ++k) {
+                            uint32_t packed[16];
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            const float e0 = exp2_fast(fmaf(x[32 * k + e], c, -base)), e1 = exp2_fast(fmaf(x[32 * k + e + 1], c, -base));
-                            const float e2 = exp2_fast(fmaf(x[32 * k + e + 2], c, -base)), e3 = exp2_fast(fmaf(x[32 * k + e + 3], c, -base));
-                            p0 += e0;
-                            p1 += e1;
-                            p2 += e2;
-                            p3 += e3;
-                            packed[e / 2] = pack2<T>(e0, e1);
-                            packed[e / 2 + 1] = pack2<T>(e2, e3);
+                            for (int e = 0; e < 32; e += 4) {
+                                const float2 f0 = split(fma2(two(x[32 * k + e], x[32 * k + e + 1]), c2, base2));
+                                const float2 f1 = split(fma2(two(x[32 * k + e + 2], x[32 * k + e + 3]), c2, base2));
+                                const float2 e0 = make_float2(exp2_fast(f0.x), exp2_fast(f0.y));
+                                const float2 e1 = decltype(by_hand)::value && (e / 4) % 4 < kByHand ? exp2_two(f1) : make_float2(exp2_fast(f1.x), exp2_fast(f1.y));
+                                s0 = add2(s0, two(e0.x, e0.y));
+                                s1 = add2(s1, two(e1.x, e1.y));
+                                packed[e / 2] = pack2<T>(e0.x, e0.y);
+                                packed[e / 2 + 1] = pack2<T>(e1.x, e1.y);
+                            }
+                            tmem_st16(t_x + 16 * k, packed);
                         }
-                        tmem_st16(t_s + 16 * k, packed);
-                    }
-                    sum += (p0 + p1) + (p2 + p3);
+                    };
+                    if (plain) weights(std::true_type{});
+                    else weights(std::false_type{});
+                    const float2 s01 = split(add2(s0, s1));
+                    sum += s01.x + s01.y;
                     tmem_wait_st();
+                }
+                const int keys = j.keys - unit * kHalf;
+                if (keys < kHalf && (keys & 15)) {
+                    // Rows of V behind the last key hold whatever their page holds, and a weight of zero does not silence an
+                    // infinity: clear what the product's last step would read.  (A pair's streams both do; they write the same.)
+                    // They are there: the S product of such a unit waits for them too.
+                    const int rows = 16 - (keys & 15);
+                    const uint32_t at = v_at + s_last[s][i % (2 * kJobs)] * S::kTileBytes + ((unit & 1) * kHalf + keys) * 128;
+#pragma unroll 1
+                    for (int e = row; e < rows * 8; e += 128) {
+#pragma unroll
+                        for (int h = 0; h < kHalves; ++h)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + h * kHalfBytes + e * 16), "r"(0) : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(b_p);
+                if (lane == 0) mbar_arrive(b_p + 8 * buf);
             }
             if (!ok) break;
             // ---- the range's result: into the output when it is all there is, else by row (an item's first
             // range) or by stream (one that continues)
-            ok = wait(b_o, (count - 1) & 1, gave_up);
+            ok = wait(b_o + 8 * ((count - 1) & 1), (count - 1) >> 1 & 1, gave_up);
             if (!ok) break;
             fence_after();
             if (!warp_on) continue;
             uint8_t* out = nullptr;
             float f = 1.f;
-            if (tok_in_tile < j.tokens) {
+            if (mine) {
                 uint8_t* ws = (uint8_t*)a.workspace;
                 const uint32_t head = j.head * group + head_in_group;
                 const uint64_t row_at = (uint64_t)tok * a.q_heads + head;
@@ -584,50 +698,56 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
                     *((float2*)(ws + (home ? w.home_ml : w.part_ml)) + at) = make_float2(top == -INFINITY ? -INFINITY : top * c, sum);
                 }
             }
-            float o[DP];
+#pragma unroll 1
+            for (int k = 0; k < DP; k += 64) {
+                float o[64];
+                tmem_ld32((uint32_t*)o, t_o + k);
+                tmem_ld32((uint32_t*)o + 32, t_o + k + 32);
+                tmem_wait_ld();
+                if (!out) continue;
+                const int left_e = (int)a.head_dim - k;                           // a multiple of 8
+                if (j.place == kPlaceDirect) {
 #pragma unroll
-            for (int k = 0; k < DP; k += 32) tmem_ld32((uint32_t*)o + k, t_o + k);
-            tmem_wait_ld();
-            fence_before();
-            if (!out) continue;
-            if (j.place == kPlaceDirect) {
+                    for (int e = 0; e < 64; e += 8)
+                        if (e < left_e)
+                            *(uint4*)(out + 2 * (k + e)) = make_uint4(pack2<T>(o[e] * f, o[e + 1] * f), pack2<T>(o[e + 2] * f, o[e + 3] * f),
+                                                                      pack2<T>(o[e + 4] * f, o[e + 5] * f), pack2<T>(o[e + 6] * f, o[e + 7] * f));
+                } else {
 #pragma unroll
-                for (int e = 0; e < DP; e += 8)
-                    if (e < (int)a.head_dim)                                      // a multiple of 8
-                        *(uint4*)(out + 2 * e) = make_uint4(pack2<T>(o[e] * f, o[e + 1] * f), pack2<T>(o[e + 2] * f, o[e + 3] * f),
-                                                            pack2<T>(o[e + 4] * f, o[e + 5] * f), pack2<T>(o[e + 6] * f, o[e + 7] * f));
-            } else {
-#pragma unroll
-                for (int e = 0; e < DP; e += 4)
-                    if (e < (int)a.head_dim) *(float4*)(out + 4 * e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int e = 0; e < 64; e += 4)
+                        if (e < left_e) *(float4*)(out + 4 * (k + e)) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
             }
+            fence_before();
         }
+    }
+    if (*gave_up) {              // what is in flight lands before the CTA ends
+        const unsigned long long t0 = now();
+        while (now() - t0 < kDrainNs) {}
     }
     fence_before();
     __syncthreads();
     if (tid == 0 && *gave_up) atomicOr(p.status, TSW_KV_WAIT_GAVE_UP);
-    if (warp == 10) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp == kWarpSchedule) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 // ---------------------------------------------------------------------------------------------
-// Joining the partial results of a row: one warp per row, four elements of the head to a lane.  The
-// ranges are visited in order, so the result does not depend on which finished first.
-constexpr int kJoinWarps = 4;
+// Joining the partial results of a row.  A block takes some heads of one token: each lane finds where the parts of one
+// head lie (the same in every warp), then each warp joins heads of its own.  Lanes take the parts' maxima and
+// sums side by side, and four elements of the head each in the sum over the parts, which goes in the
+// order of the ranges: the result does not depend on which finished first.  Everything up to the parts'
+// places is worked out while the tile kernel still runs.
+constexpr int kJoinHeads = 32;                   // heads of a block at most: one to a lane
 template <typename T>
-__global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_constant__ tsw_prefix_attention_args a, const __grid_constant__ Deal d) {
-    const int lane = threadIdx.x & 31;
-    const uint64_t row = (uint64_t)blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (row >= (uint64_t)a.batch.tokens * a.q_heads) return;
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ tsw_prefix_attention_args a, const __grid_constant__ Deal d, uint32_t heads_per_block) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int tok = (int)blockIdx.x, head0 = (int)(blockIdx.y * heads_per_block), heads = min((int)heads_per_block, (int)a.q_heads - head0);
     const AttentionLayout& w = d.w;
-    const int tok = (int)(row / a.q_heads), head = (int)(row % a.q_heads), kv_head = head / w.group;
     const int b = find_sequence((const int*)a.batch.cu_q, a.batch.batch, tok);
     if (b < 0) return;
     SeqRows r;
     read_rows(a.batch, b, a.max_q, a.cache.page_size, r);
     if (tok >= r.first + r.n) return;
-    const uint8_t* ws = (const uint8_t*)a.workspace;
-    const uint32_t* base = (const uint32_t*)(ws + w.own_base);
     uint32_t before = 0;
     for (int rt = (tok - r.first) / own_item_tokens(d), i = lane; i < rt; i += 32) {
         const Cut c = cut_own(d, r, i);
@@ -635,42 +755,77 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_c
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(~0u, before, o);
-    const Parts parts[2] = {prefix_parts(d, tok, kv_head, base[a.batch.batch + 1]),
-                            own_parts(d, r, tok, kv_head, base[b], before, base[a.batch.batch])};
-    if (!a.prefix_len && parts[1].has && parts[1].first == parts[1].last) return;      // the tile kernel has written this row itself
-    float top = -INFINITY, sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    const bool on = 4 * lane < (int)a.head_dim;
-    auto take = [&](const float2 ml, const float* o) {
-        if (ml.x == -INFINITY && ml.y == 0.f) return;
-        const float next = fmaxf(top, ml.x), base_ = next == -INFINITY ? 0.f : next;
-        const float keep = exp2f(top - base_), f = exp2f(ml.x - base_);
-        top = next;
-        sum = sum * keep + ml.y * f;
-        const float4 v = on ? *(const float4*)(o + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-        acc.x = acc.x * keep + v.x * f;
-        acc.y = acc.y * keep + v.y * f;
-        acc.z = acc.z * keep + v.z * f;
-        acc.w = acc.w * keep + v.w * f;
-    };
+    const int my_head = head0 + min(lane, heads - 1), kv_head = my_head / w.group;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint8_t* ws = (const uint8_t*)a.workspace;
+    const uint32_t* base = (const uint32_t*)(ws + w.own_base);
+    const Parts pre = prefix_parts(d, tok, kv_head, base[a.batch.batch + 1]);
+    const Parts own = own_parts(d, r, tok, kv_head, base[b], before, base[a.batch.batch]);
+    const bool direct = !a.prefix_len && own.has && own.first == own.last;      // the tile kernel has written this row itself
+    uint32_t todo = __ballot_sync(~0u, lane < heads && !direct);
+    // heads of this warp: every warps-th of them
+    for (int h = warp; h < heads; h += warps) {
+        if (!(todo >> h & 1)) continue;
+        Parts q[2];
 #pragma unroll
-    for (int l = 0; l < 2; ++l) {
-        const Parts& q = parts[l];
-        if (!q.has) continue;
-        const uint64_t home = home_index(d, l, row, a.q_heads);
-        take(((const float2*)(ws + w.home_ml))[home], (const float*)(ws + w.home_o) + home * a.head_dim);
-        const bool pair = l ? w.own_pair : w.prefix_pair;
-        for (uint32_t i = q.first + 1; i <= q.last; ++i) {
-            const uint64_t at = part_index(d, l, part_place(pair, i, q.half), q.place * w.group + head % w.group);
-            take(((const float2*)(ws + w.part_ml))[at], (const float*)(ws + w.part_o) + at * a.head_dim);
+        for (int l = 0; l < 2; ++l) {
+            const Parts& m = l ? own : pre;
+            q[l].has = __shfl_sync(~0u, (int)m.has, h);
+            q[l].first = __shfl_sync(~0u, m.first, h);
+            q[l].last = __shfl_sync(~0u, m.last, h);
+            q[l].half = __shfl_sync(~0u, m.half, h);
+            q[l].place = __shfl_sync(~0u, m.place, h);
         }
+        const int head = head0 + h, n0 = q[0].has ? (int)(q[0].last - q[0].first) + 1 : 0, n = n0 + (q[1].has ? (int)(q[1].last - q[1].first) + 1 : 0);
+        const uint64_t row = (uint64_t)tok * a.q_heads + head;
+        // The i-th part: of the prefix list first, in each list the one by row, then those of the ranges that continue.
+        auto part = [&](int i, const float2*& ml, const float*& o) {
+            const int l = i >= n0, k = i - (l ? n0 : 0);
+            const bool pair = l ? w.own_pair : w.prefix_pair;
+            const uint32_t place = (l ? q[1].place : q[0].place) * w.group + head % w.group, range = (l ? q[1].first : q[0].first) + k;
+            const uint64_t at = k ? part_index(d, l, part_place(pair, range, l ? q[1].half : q[0].half), place) : home_index(d, l, row, a.q_heads);
+            ml = (const float2*)(ws + (k ? w.part_ml : w.home_ml)) + at;
+            o = (const float*)(ws + (k ? w.part_o : w.home_o)) + at * a.head_dim;
+        };
+        float top = -INFINITY, sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        const bool on = 4 * lane < (int)a.head_dim;
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            const float2* ml;
+            const float* o;
+            float2 mine = make_float2(-INFINITY, 0.f);
+            if (i0 + lane < n) {
+                part(i0 + lane, ml, o);
+                mine = *ml;
+            }
+            const float next = fmaxf(top, warp_max(mine.x)), base_m = next == -INFINITY ? 0.f : next;
+            const float keep = exp2f(top - base_m), f = mine.x == -INFINITY && mine.y == 0.f ? 0.f : exp2f(mine.x - base_m);
+            top = next;
+            sum = sum * keep + warp_sum(mine.y * f);
+            acc.x *= keep;
+            acc.y *= keep;
+            acc.z *= keep;
+            acc.w *= keep;
+            const int m = min(32, n - i0);
+#pragma unroll 4
+            for (int i = 0; i < m; ++i) {
+                const float fi = __shfl_sync(~0u, f, i);
+                part(i0 + i, ml, o);
+                if (!on) continue;
+                const float4 v = *(const float4*)(o + 4 * lane);
+                acc.x = fmaf(v.x, fi, acc.x);
+                acc.y = fmaf(v.y, fi, acc.y);
+                acc.z = fmaf(v.z, fi, acc.z);
+                acc.w = fmaf(v.w, fi, acc.w);
+            }
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        if (on) {
+            const uint2 v = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+            *(uint2*)(a.out + (uint64_t)tok * a.out_token_stride + (uint64_t)head * a.out_head_stride + 8 * lane) = v;
+        }
+        if (a.lse && lane == 0) ((float*)a.lse)[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (on) {
-        const uint2 v = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-        *(uint2*)(a.out + (uint64_t)tok * a.out_token_stride + (uint64_t)head * a.out_head_stride + 8 * lane) = v;
-    }
-    if (a.lse && lane == 0) ((float*)a.lse)[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 // ------------------------------------------------------------------------------------- host
@@ -736,10 +891,13 @@ cudaError_t launch_tiles(const Params& p, cudaStream_t stream) {
     early.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &early;
     cfg.numAttrs = 1;
-    cfg.gridDim = dim3((unsigned)(((uint64_t)p.a.batch.tokens * p.a.q_heads + kJoinWarps - 1) / kJoinWarps));
-    cfg.blockDim = dim3(32 * kJoinWarps);
+    // Few tokens: few heads to a block, so that every warp has one; many: a block takes up to 32 heads.
+    const uint32_t rows = p.a.q_heads, most = std::min<uint32_t>(rows, kJoinHeads);
+    const uint32_t per = std::min(most, std::max(4u, (uint32_t)((uint64_t)p.a.batch.tokens * rows / (8u * p.d.w.ctas))));
+    cfg.gridDim = dim3(p.a.batch.tokens, (rows + per - 1) / per);
+    cfg.blockDim = dim3(32 * std::min(8u, per));
     cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, combine_kernel<T>, p.a, p.d);
+    return cudaLaunchKernelEx(&cfg, combine_kernel<T>, p.a, p.d, per);
 }
 
 }  // namespace

@@ -311,17 +311,42 @@ struct Walk {
     }
 };
 
-// What the warps are told.  A unit is one key tile for one stream; the two units of a pair's tile share one load.
-struct alignas(16) Unit {
-    uint32_t flags;          // kUnit*, keys of the tile from bit 8, key head from bit 16
+// What the warps are told.  A load is one key tile for the loading warps.  A take is the same tile for the products of one
+// stream; of a list that is dealt in pairs each stream is told of every tile, also of those that it has no product
+// with.  Products go by half tiles (units); a half that lies behind the last key is none.
+constexpr int kHalf = kTile / 2;
+struct alignas(16) Load {
+    uint32_t flags;          // kLoad*, keys of the tile from bit 8, key head from bit 16
     int tile, b, pad;
 };
-enum { kUnitStream = 1, kUnitLoad = 2, kUnitRelease = 4, kUnitFirst = 8, kUnitOwn = 16, kUnitEnd = 32 };
-TSW_HD int unit_keys(uint32_t flags) { return (flags >> 8 & 0xff) + 1; }
-TSW_HD int unit_head(uint32_t flags) { return flags >> 16; }
-// A stream's share of a job: its rows, how many tiles, and where the result goes.
+enum { kLoadOwn = 1, kLoadEnd = 2, kLoadPair = 4, kLoadSecond = 8 };      // Second: the second stream's, of a list that is not in pairs
+TSW_HD int load_keys(uint32_t flags) { return (flags >> 8 & 0xff) + 1; }
+TSW_HD int load_head(uint32_t flags) { return flags >> 16; }
+TSW_HD int tile_keys(const Job& j, int tile) { return imin(kTile, j.keys - tile * kTile); }
+TSW_HD Load make_load(const Job& j, int tile, bool pair, bool use1) {
+    return Load{(j.own ? kLoadOwn : 0u) | (pair ? kLoadPair : use1 ? kLoadSecond : 0u) | (uint32_t)(tile_keys(j, tile) - 1) << 8 | (uint32_t)j.head << 16, tile, j.b, 0};
+}
+struct Ring {                // place in a ring of n slots
+    uint32_t slot, phase;
+    TSW_HD void step(uint32_t n) {
+        if (++slot == n) {
+            slot = 0;
+            phase ^= 1;
+        }
+    }
+};
+// Bits of a take: kTake*, the tile's keys from bit 8, the slots of its keys and values from bits 16 and 24.
+enum { kTakeFirst = 1, kTakeSkip = 2, kTakePair = 4, kTakeEnd = 8 };
+TSW_HD int take_keys(uint32_t u) { return (u >> 8 & 0xff) + 1; }
+TSW_HD uint32_t k_slot(uint32_t u) { return u >> 16 & 0xff; }
+TSW_HD uint32_t v_slot(uint32_t u) { return u >> 24; }
+TSW_HD int units_of(int keys) { return keys > kHalf ? 2 : 1; }
+TSW_HD uint32_t make_take(const Job& j, int tile, bool use, bool pair, uint32_t k, uint32_t v) {
+    return (tile == j.kt0 ? kTakeFirst : 0u) | (use ? 0u : kTakeSkip) | (pair ? kTakePair : 0u) | (uint32_t)(tile_keys(j, tile) - 1) << 8 | k << 16 | v << 24;
+}
+// A stream's share of a job: its rows, how many units, and where the result goes.
 struct alignas(16) RowJob {
-    int head, tok, tokens, tiles;    // tiles = 0: no more
+    int head, tok, tokens, units;    // units = 0: no more
     int keys, limit;                 // from the range's first key: row of token t sees keys below min(keys, limit + t)
     int own, place;                  // place >= 0: partial result of a range that continues an item
 };
@@ -329,23 +354,13 @@ enum { kPlaceDirect = -2, kPlaceHome = -1 };
 
 // End of what stream s sees of the job's keys (pairs: each row tile its own).
 TSW_HD int seen_by(const Job& j, bool pair, int s) { return pair && s ? j.kt_b : j.kt_a; }
-TSW_HD Unit make_unit(const Job& j, int tile, int s, bool use0, bool use1) {
-    Unit u;
-    const int keys = imin(kTile, j.keys - tile * kTile);
-    u.flags = (s ? kUnitStream : 0) | (s && use0 ? 0 : kUnitLoad) | (!s && use1 ? 0 : kUnitRelease) | (tile == j.kt0 ? kUnitFirst : 0) |
-              (j.own ? kUnitOwn : 0) | (uint32_t)(keys - 1) << 8 | (uint32_t)j.head << 16;
-    u.tile = tile;
-    u.b = j.b;
-    u.pad = 0;
-    return u;
-}
 TSW_HD RowJob make_row_job(const Deal& d, const Job& j, bool pair, int s, uint32_t cta) {
     RowJob r;
     const int seen = seen_by(j, pair, s), end = imin(j.kt1, seen);
     r.head = j.head;
     r.tok = j.tok + (pair && s ? (int)d.w.tile_tokens : 0);
     r.tokens = pair && s ? j.n_b : j.n_a;
-    r.tiles = end - j.kt0;
+    r.units = 2 * (end - j.kt0 - 1) + units_of(tile_keys(j, end - 1));
     r.keys = j.keys - j.kt0 * kTile;
     r.limit = j.limit + 1 - j.kt0 * kTile;
     r.own = j.own;
