@@ -732,16 +732,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
 }
 
 // ---------------------------------------------------------------------------------------------
-// Joining the partial results of a row.  A block takes some heads of one token: each lane finds where the parts of one
-// head lie (the same in every warp), then each warp joins heads of its own.  Lanes take the parts' maxima and
-// sums side by side, and four elements of the head each in the sum over the parts, which goes in the
-// order of the ranges: the result does not depend on which finished first.  Everything up to the parts'
-// places is worked out while the tile kernel still runs.
-constexpr int kJoinHeads = 32;                   // heads of a block at most: one to a lane
-template <typename T>
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ tsw_prefix_attention_args a, const __grid_constant__ Deal d, uint32_t heads_per_block) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int tok = (int)blockIdx.x, head0 = (int)(blockIdx.y * heads_per_block), heads = min((int)heads_per_block, (int)a.q_heads - head0);
+// Joining the partial results of a row: eight lanes to a row, four rows (heads of one token) to a warp, so that
+// a warp has many loads under way: the work is a handful of dependent loads to a row, not arithmetic.  The lanes take
+// the parts' maxima and sums side by side, and DP / 8 elements of the head each in the sum over the parts, which
+// goes in the order of the ranges: the result does not depend on which finished first.  What does not come from the tile
+// kernel is worked out while it still runs.
+constexpr int kJoinThreads = 128;
+template <typename T, int DP>
+__global__ void __launch_bounds__(kJoinThreads) combine_kernel(const __grid_constant__ tsw_prefix_attention_args a, const __grid_constant__ Deal d) {
+    constexpr int kVec = DP / 32;                    // float4s of a lane: element 4 * (sub + 8 * i)
+    const int lane = threadIdx.x & 31, sub = lane & 7;
+    const int tok = (int)blockIdx.x, head = (int)(blockIdx.y * (kJoinThreads / 8) + threadIdx.x / 8);
     const AttentionLayout& w = d.w;
     const int b = find_sequence((const int*)a.batch.cu_q, a.batch.batch, tok);
     if (b < 0) return;
@@ -755,77 +756,88 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ ts
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(~0u, before, o);
-    const int my_head = head0 + min(lane, heads - 1), kv_head = my_head / w.group;
+    const int kv_head = min(head, (int)a.q_heads - 1) / w.group;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint8_t* ws = (const uint8_t*)a.workspace;
     const uint32_t* base = (const uint32_t*)(ws + w.own_base);
-    const Parts pre = prefix_parts(d, tok, kv_head, base[a.batch.batch + 1]);
     const Parts own = own_parts(d, r, tok, kv_head, base[b], before, base[a.batch.batch]);
-    const bool direct = !a.prefix_len && own.has && own.first == own.last;      // the tile kernel has written this row itself
-    uint32_t todo = __ballot_sync(~0u, lane < heads && !direct);
-    // heads of this warp: every warps-th of them
-    for (int h = warp; h < heads; h += warps) {
-        if (!(todo >> h & 1)) continue;
-        Parts q[2];
+    Parts pre = {};
+    if (a.prefix_len) pre = prefix_parts(d, tok, kv_head, base[a.batch.batch + 1]);
+    // without a prefix, a row that one range holds has been written by the tile kernel itself
+    const bool on = head < (int)a.q_heads && (a.prefix_len || !own.has || own.first != own.last);
+    if (!__any_sync(~0u, on)) return;
+    const int n0 = on && pre.has ? (int)(pre.last - pre.first) + 1 : 0, n = n0 + (on && own.has ? (int)(own.last - own.first) + 1 : 0);
+    int most = n;
+    most = max(most, __shfl_xor_sync(~0u, most, 8));
+    most = max(most, __shfl_xor_sync(~0u, most, 16));
+    const uint64_t row = (uint64_t)tok * a.q_heads + head;
+    // The i-th part: of the prefix list first, in each list the one by row, then those of the ranges that continue.
+    const uint32_t in_group = head % w.group;
+    const uint64_t home0 = home_index(d, 0, row, a.q_heads), home1 = home_index(d, 1, row, a.q_heads);
+    auto part = [&](int i) -> uint64_t {             // its place; bit 63: among those of the ranges that continue
+        const bool l = i >= n0;
+        const int k = l ? i - n0 : i;
+        if (k == 0) return l ? home1 : home0;
+        const Parts& q = l ? own : pre;
+        return part_index(d, l, part_place(l ? w.own_pair : w.prefix_pair, q.first + k, q.half), q.place * w.group + in_group) | 1ull << 63;
+    };
+    float top = -INFINITY, sum = 0.f;
+    float4 acc[kVec];
 #pragma unroll
-        for (int l = 0; l < 2; ++l) {
-            const Parts& m = l ? own : pre;
-            q[l].has = __shfl_sync(~0u, (int)m.has, h);
-            q[l].first = __shfl_sync(~0u, m.first, h);
-            q[l].last = __shfl_sync(~0u, m.last, h);
-            q[l].half = __shfl_sync(~0u, m.half, h);
-            q[l].place = __shfl_sync(~0u, m.place, h);
+    for (int e = 0; e < kVec; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < most; i0 += 8) {
+        float2 mine = make_float2(-INFINITY, 0.f);
+        uint64_t at = 0;
+        if (i0 + sub < n) {
+            at = part(i0 + sub);
+            mine = ((const float2*)(ws + (at >> 63 ? w.part_ml : w.home_ml)))[at & ~(1ull << 63)];
         }
-        const int head = head0 + h, n0 = q[0].has ? (int)(q[0].last - q[0].first) + 1 : 0, n = n0 + (q[1].has ? (int)(q[1].last - q[1].first) + 1 : 0);
-        const uint64_t row = (uint64_t)tok * a.q_heads + head;
-        // The i-th part: of the prefix list first, in each list the one by row, then those of the ranges that continue.
-        auto part = [&](int i, const float2*& ml, const float*& o) {
-            const int l = i >= n0, k = i - (l ? n0 : 0);
-            const bool pair = l ? w.own_pair : w.prefix_pair;
-            const uint32_t place = (l ? q[1].place : q[0].place) * w.group + head % w.group, range = (l ? q[1].first : q[0].first) + k;
-            const uint64_t at = k ? part_index(d, l, part_place(pair, range, l ? q[1].half : q[0].half), place) : home_index(d, l, row, a.q_heads);
-            ml = (const float2*)(ws + (k ? w.part_ml : w.home_ml)) + at;
-            o = (const float*)(ws + (k ? w.part_o : w.home_o)) + at * a.head_dim;
-        };
-        float top = -INFINITY, sum = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        const bool on = 4 * lane < (int)a.head_dim;
-        for (int i0 = 0; i0 < n; i0 += 32) {
-            const float2* ml;
-            const float* o;
-            float2 mine = make_float2(-INFINITY, 0.f);
-            if (i0 + lane < n) {
-                part(i0 + lane, ml, o);
-                mine = *ml;
-            }
-            const float next = fmaxf(top, warp_max(mine.x)), base_m = next == -INFINITY ? 0.f : next;
-            const float keep = exp2f(top - base_m), f = mine.x == -INFINITY && mine.y == 0.f ? 0.f : exp2f(mine.x - base_m);
-            top = next;
-            sum = sum * keep + warp_sum(mine.y * f);
-            acc.x *= keep;
-            acc.y *= keep;
-            acc.z *= keep;
-            acc.w *= keep;
-            const int m = min(32, n - i0);
-#pragma unroll 4
-            for (int i = 0; i < m; ++i) {
-                const float fi = __shfl_sync(~0u, f, i);
-                part(i0 + i, ml, o);
-                if (!on) continue;
-                const float4 v = *(const float4*)(o + 4 * lane);
-                acc.x = fmaf(v.x, fi, acc.x);
-                acc.y = fmaf(v.y, fi, acc.y);
-                acc.z = fmaf(v.z, fi, acc.z);
-                acc.w = fmaf(v.w, fi, acc.w);
+        float next = fmaxf(top, mine.x);
+#pragma unroll
+        for (int o = 4; o; o >>= 1) next = fmaxf(next, __shfl_xor_sync(~0u, next, o));
+        const float base_m = next == -INFINITY ? 0.f : next;
+        const float keep = exp2f(top - base_m), f = mine.x == -INFINITY && mine.y == 0.f ? 0.f : exp2f(mine.x - base_m);
+        float add = mine.y * f;
+#pragma unroll
+        for (int o = 4; o; o >>= 1) add += __shfl_xor_sync(~0u, add, o);
+        top = next;
+        sum = sum * keep + add;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+            acc[e].x *= keep;
+            acc[e].y *= keep;
+            acc[e].z *= keep;
+            acc[e].w *= keep;
+        }
+        const int m = min(8, most - i0);
+#pragma unroll 2
+        for (int i = 0; i < m; ++i) {
+            const float fi = __shfl_sync(~0u, f, (lane & 24) + i);
+            const uint64_t from = __shfl_sync(~0u, at, (lane & 24) + i);
+            if (i0 + i >= n) continue;
+            const float* o = (const float*)(ws + (from >> 63 ? w.part_o : w.home_o)) + (from & ~(1ull << 63)) * a.head_dim;
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) {
+                const int at_e = 4 * (sub + 8 * e);
+                if (at_e >= (int)a.head_dim) continue;
+                const float4 v = *(const float4*)(o + at_e);
+                acc[e].x = fmaf(v.x, fi, acc[e].x);
+                acc[e].y = fmaf(v.y, fi, acc[e].y);
+                acc[e].z = fmaf(v.z, fi, acc[e].z);
+                acc[e].w = fmaf(v.w, fi, acc[e].w);
             }
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        if (on) {
-            const uint2 v = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-            *(uint2*)(a.out + (uint64_t)tok * a.out_token_stride + (uint64_t)head * a.out_head_stride + 8 * lane) = v;
-        }
-        if (a.lse && lane == 0) ((float*)a.lse)[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
     }
+    if (!on) return;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+        const int at_e = 4 * (sub + 8 * e);
+        if (at_e >= (int)a.head_dim) continue;
+        const uint2 v = make_uint2(pack2<T>(acc[e].x * inv, acc[e].y * inv), pack2<T>(acc[e].z * inv, acc[e].w * inv));
+        *(uint2*)(a.out + (uint64_t)tok * a.out_token_stride + (uint64_t)head * a.out_head_stride + 2 * at_e) = v;
+    }
+    if (a.lse && sub == 0) ((float*)a.lse)[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 // ------------------------------------------------------------------------------------- host
@@ -891,13 +903,10 @@ cudaError_t launch_tiles(const Params& p, cudaStream_t stream) {
     early.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &early;
     cfg.numAttrs = 1;
-    // Few tokens: few heads to a block, so that every warp has one; many: a block takes up to 32 heads.
-    const uint32_t rows = p.a.q_heads, most = std::min<uint32_t>(rows, kJoinHeads);
-    const uint32_t per = std::min(most, std::max(4u, (uint32_t)((uint64_t)p.a.batch.tokens * rows / (8u * p.d.w.ctas))));
-    cfg.gridDim = dim3(p.a.batch.tokens, (rows + per - 1) / per);
-    cfg.blockDim = dim3(32 * std::min(8u, per));
+    cfg.gridDim = dim3(p.a.batch.tokens, (p.a.q_heads + kJoinThreads / 8 - 1) / (kJoinThreads / 8));
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, combine_kernel<T>, p.a, p.d, per);
+    return cudaLaunchKernelEx(&cfg, combine_kernel<T, DP>, p.a, p.d);
 }
 
 }  // namespace
