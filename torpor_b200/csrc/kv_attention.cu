@@ -35,7 +35,6 @@ namespace {
 
 constexpr int kThreads = 416;                 // two warpgroups of rows; warps for keys, values, each stream's products, scheduling
 constexpr unsigned long long kWaitNs = 2000000000ull, kDrainNs = 5000000ull;
-constexpr int kByHand = 0;                    // of 8 pairs of exponentials
 constexpr float kGrow = 8.f;                  // log2 of the growth of the maximum that is let pass
 
 template <int DP> struct Shape {
@@ -182,24 +181,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
-}
-// 2^x of two numbers without the special function unit, for finite x <= 8 (or below: 2^-125 at least comes back).  x is
-// split into the nearest integer, which goes into the exponent, and a rest in [-1/2, 1/2], where a polynomial of
-// degree 5 fitted to the least relative error (Remez exchange) is within 2^-23 of 2^rest.
-__device__ __forceinline__ float2 exp2_two(float2 x) {
-    constexpr float kRound = 12582912.f;                 // 1.5 * 2^23: adding it rounds to an integer, kept in the low bits
-    const uint64_t v = two(fmaxf(x.x, -125.f), fmaxf(x.y, -125.f));
-    const uint64_t t = add2(v, two(kRound, kRound));
-    const uint64_t f = fma2(add2(t, two(-kRound, -kRound)), two(-1.f, -1.f), v);
-    uint64_t p = two(1.3276472454890609e-3f, 1.3276472454890609e-3f);
-    p = fma2(p, f, two(9.675540961325169e-3f, 9.675540961325169e-3f));
-    p = fma2(p, f, two(5.550713092088699e-2f, 5.550713092088699e-2f));
-    p = fma2(p, f, two(0.24022120237350464f, 0.24022120237350464f));
-    p = fma2(p, f, two(0.6931469440460205f, 0.6931469440460205f));
-    p = fma2(p, f, two(1.0000001192092896f, 1.0000001192092896f));
-    const float2 n = split(t), m = split(p);
-    return make_float2(__uint_as_float((__float_as_uint(n.x) << 23) + __float_as_uint(m.x)),
-                       __uint_as_float((__float_as_uint(n.y) << 23) + __float_as_uint(m.y)));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
@@ -627,30 +608,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
                     const float base = top == -INFINITY ? 0.f : top * c;
                     const uint64_t c2 = two(c, c), base2 = two(-base, -base);
                     uint64_t s0 = 0, s1 = 0;
-                    // Two warps of a scheduler share a special function unit that takes 8 cycles an instruction: 1024 cycles for
-                    // their 64 columns each, against 512 of products.  Where nothing is masked and all scores are finite,
-                    // kByHand of 8 pairs are formed by multiplications instead.
-                    const bool plain = __all_sync(~0u, !mine || (left >= kHalf && fabsf(here) < INFINITY));
-                    auto weights = [&](auto by_hand) {
 #pragma unroll
-                        for (int k = 0; k < kHalf / 32; ++k) {
-                            uint32_t packed[16];
+                    for (int k = 0; k < kHalf / 32; ++k) {
+                        uint32_t packed[16];
 #pragma unroll
-                            for (int e = 0; e < 32; e += 4) {
-                                const float2 f0 = split(fma2(two(x[32 * k + e], x[32 * k + e + 1]), c2, base2));
-                                const float2 f1 = split(fma2(two(x[32 * k + e + 2], x[32 * k + e + 3]), c2, base2));
-                                const float2 e0 = make_float2(exp2_fast(f0.x), exp2_fast(f0.y));
-                                const float2 e1 = decltype(by_hand)::value && (e / 4) % 4 < kByHand ? exp2_two(f1) : make_float2(exp2_fast(f1.x), exp2_fast(f1.y));
-                                s0 = add2(s0, two(e0.x, e0.y));
-                                s1 = add2(s1, two(e1.x, e1.y));
-                                packed[e / 2] = pack2<T>(e0.x, e0.y);
-                                packed[e / 2 + 1] = pack2<T>(e1.x, e1.y);
-                            }
-                            tmem_st16(t_x + 16 * k, packed);
+                        for (int e = 0; e < 32; e += 4) {
+                            const float2 f0 = split(fma2(two(x[32 * k + e], x[32 * k + e + 1]), c2, base2));
+                            const float2 f1 = split(fma2(two(x[32 * k + e + 2], x[32 * k + e + 3]), c2, base2));
+                            const float e0 = exp2_fast(f0.x), e1 = exp2_fast(f0.y), e2 = exp2_fast(f1.x), e3 = exp2_fast(f1.y);
+                            s0 = add2(s0, two(e0, e1));
+                            s1 = add2(s1, two(e2, e3));
+                            packed[e / 2] = pack2<T>(e0, e1);
+                            packed[e / 2 + 1] = pack2<T>(e2, e3);
                         }
-                    };
-                    if (plain) weights(std::true_type{});
-                    else weights(std::false_type{});
+                        tmem_st16(t_x + 16 * k, packed);
+                    }
                     const float2 s01 = split(add2(s0, s1));
                     sum += s01.x + s01.y;
                     tmem_wait_st();

@@ -11,8 +11,10 @@
 
 #ifdef __CUDACC__
 #define TSW_HD __host__ __device__ __forceinline__
+#define TSW_HD_CALL __host__ __device__ __noinline__      // one copy: the kernels' code is fetched cold at every launch
 #else
 #define TSW_HD inline
+#define TSW_HD_CALL
 #endif
 
 namespace tsw {
@@ -123,7 +125,7 @@ TSW_HD Cut cut_own(const Deal& d, const SeqRows& r, int rt) {
     c.kt_b = c.n_b ? tiles_of(d.causal ? imax(0, imin(r.len, past + left)) : r.len) : 0;
     return c;
 }
-TSW_HD uint32_t sequence_tiles(const Deal& d, const SeqRows& r) {     // over all key heads
+TSW_HD_CALL inline uint32_t sequence_tiles(const Deal& d, const SeqRows& r) {     // over all key heads
     uint32_t sum = 0;
     for (int rt = 0, per = own_item_tokens(d); rt * per < r.n; ++rt) {
         const Cut c = cut_own(d, r, rt);
@@ -135,8 +137,9 @@ TSW_HD uint32_t sequence_tiles(const Deal& d, const SeqRows& r) {     // over al
 // A list of `total` tiles is cut into n ranges, none of them empty; range i starts at i * total / n.  The range that
 // holds tile x; how many there are; the range of a CTA's stream (neighbours on different CTAs, so that few ranges
 // spread over many); the streams' places for partial results, numbered by range.
-TSW_HD uint32_t range_start(uint32_t i, uint32_t total, uint32_t n) { return (uint32_t)((uint64_t)i * total / n); }
-TSW_HD uint32_t range_of(uint32_t x, uint32_t total, uint32_t n) { return (uint32_t)((((uint64_t)x + 1) * n - 1) / total); }
+TSW_HD_CALL inline uint32_t quotient(uint64_t a, uint32_t b) { return (uint32_t)(a / b); }
+TSW_HD uint32_t range_start(uint32_t i, uint32_t total, uint32_t n) { return quotient((uint64_t)i * total, n); }
+TSW_HD uint32_t range_of(uint32_t x, uint32_t total, uint32_t n) { return quotient(((uint64_t)x + 1) * n - 1, total); }
 TSW_HD uint32_t ranges(const Deal& d, bool pair, uint32_t total) {
     const uint32_t n = pair ? d.w.ctas : 2 * d.w.ctas;
     return total < n ? total : n;
@@ -178,7 +181,7 @@ TSW_HD uint32_t prefix_rows(const Deal& d, int& tok0, int& tok1) {      // row t
     return (uint32_t)((tok1 - tok0 + per - 1) / per);
 }
 // Tile `off` of the own tiles of sequences [lo, hi) begins a range of `left` tiles.
-TSW_HD bool find_start(const Deal& d, int lo, int hi, uint32_t off, uint32_t left, Start& s) {
+TSW_HD_CALL inline bool find_start(const Deal& d, int lo, int hi, uint32_t off, uint32_t left, Start& s) {
     for (int b = lo; b < hi; ++b) {
         SeqRows r;
         read_rows(d.batch, b, d.max_q, d.page_size, r);
