@@ -860,9 +860,14 @@ cudaError_t encode_queries(CUtensorMap* map, const tsw_prefix_attention_args& a,
 }
 
 template <typename T, int DP>
-cudaError_t launch_tiles(const Params& p, cudaStream_t stream) {
-    cudaError_t err = cudaFuncSetAttribute(attention_tiles_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP>::kSmem);
-    if (err != cudaSuccess) return err;
+cudaError_t launch_tiles(int device, const Params& p, cudaStream_t stream) {
+    static std::atomic<uint64_t> ready{0};          // devices on which the kernel has been given its shared memory
+    cudaError_t err = cudaSuccess;
+    if (!(ready.load(std::memory_order_relaxed) >> device & 1)) {
+        err = cudaFuncSetAttribute(attention_tiles_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP>::kSmem);
+        if (err != cudaSuccess) return err;
+        ready.fetch_or(1ull << device, std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.d.w.ctas);
     cfg.blockDim = dim3(kThreads);
@@ -883,7 +888,7 @@ cudaError_t launch_tiles(const Params& p, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t launch_prefix_attention_tiles(const tsw_prefix_attention_args& a, const AttentionLayout& w, uint32_t* status, cudaStream_t stream) {
+cudaError_t launch_prefix_attention_tiles(int device, const tsw_prefix_attention_args& a, const AttentionLayout& w, uint32_t* status, cudaStream_t stream) {
     Params p;
     p.a = a;
     p.d = Deal{a.batch, a.max_q, a.cache.page_size, a.kv_heads, a.prefix_len, a.causal, w};
@@ -904,8 +909,8 @@ cudaError_t launch_prefix_attention_tiles(const tsw_prefix_attention_args& a, co
     p.q_prefix = p.q_own;
     if (w.own_box_tokens != w.tile_tokens) err = encode_queries(&p.q_prefix, a, w.group, w.tile_tokens);
     if (err != cudaSuccess) return err;
-    if (a.head_dim <= 64) return a.dtype == TSW_F16 ? launch_tiles<__half, 64>(p, stream) : launch_tiles<__nv_bfloat16, 64>(p, stream);
-    return a.dtype == TSW_F16 ? launch_tiles<__half, 128>(p, stream) : launch_tiles<__nv_bfloat16, 128>(p, stream);
+    if (a.head_dim <= 64) return a.dtype == TSW_F16 ? launch_tiles<__half, 64>(device, p, stream) : launch_tiles<__nv_bfloat16, 64>(device, p, stream);
+    return a.dtype == TSW_F16 ? launch_tiles<__half, 128>(device, p, stream) : launch_tiles<__nv_bfloat16, 128>(device, p, stream);
 }
 
 }  // namespace tsw

@@ -25,7 +25,7 @@ struct AttentionLayout {
 };
 
 #ifdef __CUDART_API_VERSION
-cudaError_t launch_prefix_attention_tiles(const tsw_prefix_attention_args& a, const AttentionLayout& w, uint32_t* status, cudaStream_t stream);
+cudaError_t launch_prefix_attention_tiles(int device, const tsw_prefix_attention_args& a, const AttentionLayout& w, uint32_t* status, cudaStream_t stream);
 #endif
 
 }  // namespace tsw

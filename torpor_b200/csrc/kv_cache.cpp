@@ -16,9 +16,14 @@ constexpr int kMaxDevices = 64;
 constexpr uint32_t kMaxHeadDim = 512;
 constexpr int kMaxSms = 160;    // what a workspace is sized for before the device is known
 
-struct DeviceGuard {            // the caller's current device is put back
+struct DeviceGuard {            // makes a device current; the caller's is put back
     int old = -1;
-    DeviceGuard() { if (cudaGetDevice(&old) != cudaSuccess) old = -1; }
+    cudaError_t err;
+    explicit DeviceGuard(int device) {
+        err = cudaGetDevice(&old);
+        if (err == cudaSuccess && old == device) old = -1;
+        else if (err == cudaSuccess) err = cudaSetDevice(device);
+    }
     ~DeviceGuard() { if (old >= 0) cudaSetDevice(old); }
 };
 
@@ -139,9 +144,8 @@ int check_attention(const tsw_prefix_attention_args& a) {
     return check_rows("out", a.out, a.out_token_stride, a.out_head_stride, a.batch, a.q_heads, row, true);
 }
 
-int use_device(int device, int* sms) {
-    const cudaError_t err = cudaSetDevice(device);
-    if (err != cudaSuccess) return fail(TSW_ERR_NO_DEVICE, std::string("cudaSetDevice: ") + cudaGetErrorString(err));
+int use_device(const DeviceGuard& g, int device, int* sms) {
+    if (g.err != cudaSuccess) return fail(TSW_ERR_NO_DEVICE, std::string("cudaSetDevice: ") + cudaGetErrorString(g.err));
     return sm_count(device, sms);
 }
 
@@ -220,9 +224,9 @@ int tsw_kv_append(int device, const tsw_kv_append_args* args, void* stream) {
         if (device < 0 || device >= kMaxDevices) return bad("device ordinal out of range");
         CHECK(check_append(*args));
         if (!args->batch.tokens || !args->batch.batch) return TSW_OK;
-        DeviceGuard restore;
+        const DeviceGuard guard(device);
         int sms;
-        CHECK(use_device(device, &sms));
+        CHECK(use_device(guard, device, &sms));
         TSW_CUDA(launch_kv_append(*args, sms, (cudaStream_t)stream));
         return TSW_OK;
     });
@@ -244,9 +248,9 @@ int tsw_prefix_attention(int device, const tsw_prefix_attention_args* args, void
         if (device < 0 || device >= kMaxDevices) return bad("device ordinal out of range");
         CHECK(check_attention(*args));
         if (!args->batch.tokens || !args->batch.batch) return TSW_OK;
-        DeviceGuard restore;
+        const DeviceGuard guard(device);
         int sms;
-        CHECK(use_device(device, &sms));
+        CHECK(use_device(guard, device, &sms));
         AttentionLayout w;
         if (!attention_layout(*args, std::min(sms, kMaxSms), &w)) {
             TSW_CUDA(launch_prefix_attention_rows(*args, (cudaStream_t)stream));
@@ -256,7 +260,7 @@ int tsw_prefix_attention(int device, const tsw_prefix_attention_args* args, void
         if (args->workspace_bytes < w.bytes) return fail(TSW_ERR_BUFFER, "workspace is smaller than tsw_prefix_attention_workspace asks for");
         uint32_t* word;
         CHECK(status_word(device, &word));
-        TSW_CUDA(launch_prefix_attention_tiles(*args, w, word, (cudaStream_t)stream));
+        TSW_CUDA(launch_prefix_attention_tiles(device, *args, w, word, (cudaStream_t)stream));
         return TSW_OK;
     });
 }
@@ -265,9 +269,9 @@ int tsw_kv_status(int device, void* stream, uint32_t* status, int clear) {
     return guarded([&]() -> int {
         if (!status) return bad("null argument");
         if (device < 0 || device >= kMaxDevices) return bad("device ordinal out of range");
-        DeviceGuard restore;
+        const DeviceGuard guard(device);
         int sms;
-        CHECK(use_device(device, &sms));
+        CHECK(use_device(guard, device, &sms));
         uint32_t* word = nullptr;
         CHECK(status_word(device, &word));
         cudaStream_t s = (cudaStream_t)stream;
