@@ -410,11 +410,11 @@ int tsw_prefix_attention(int device, const tsw_prefix_attention_args* args, void
 enum { TSW_KV_BAD_PAGE = 1, TSW_KV_BAD_LENGTH = 2, TSW_KV_BAD_ROWS = 4, TSW_KV_WAIT_GAVE_UP = 8 };
 int tsw_kv_status(int device, void* stream, uint32_t* status, int clear);
 
-/* The same operators on a function's own memory: every address in `args` except workspace is a client address of
+/* The same operators on a function's own memory: every address in `args` is a client address of
  * `func` and is translated as the executor translates a kernel's arguments (cuda_server.hpp:1265-1268);
  * each operand must lie inside one block of the function (TSW_ERR_NOT_FOUND otherwise).  Parameters
  * that are still being swapped in are waited for on the stream, as in tsw_translate_async, and are recorded as
- * accessed. */
+ * accessed.  TSW_ERR_STATE when a block is not on the engine's GPU. */
 int tsw_func_kv_append(tsw_engine* e, const char* func, const tsw_kv_append_args* args, void* stream);
 int tsw_func_prefix_attention(tsw_engine* e, const char* func, const tsw_prefix_attention_args* args, void* stream);
 

@@ -181,7 +181,7 @@ int operand(tsw_engine* e, const char* func, uint64_t* addr, uint64_t bytes, con
             uint64_t phys;
             int waited;
             const uint64_t vaddr = v.vaddr;
-            tsw_mark_access(e, vaddr);
+            if (e->tracking && e->track_func == func) tsw_mark_access(e, vaddr);
             CHECK(tsw_translate_async(e, func, vaddr, stream, &phys, &waited));
         }
         *addr = pl.blocks[i].cuda + (*addr - b.vaddr);
@@ -293,20 +293,21 @@ int tsw_func_kv_append(tsw_engine* e, const char* func, const tsw_kv_append_args
         CHECK(check_append(*args));
         tsw_kv_append_args a = *args;
         const uint64_t row = 2ull * a.head_dim;
-        {
-            Lock g1(repo().mu);
-            Lock g2(e->mu);
-            CHECK(operand_pages(e, func, a.cache, row, a.kv_heads, stream));
-            CHECK(operand_batch(e, func, a.batch, stream));
-            const bool same = a.q == a.q_out;
-            CHECK(operand(e, func, &a.q, span(row, a.batch.tokens, a.q_token_stride, a.q_heads, a.q_head_stride), "q", stream));
-            if (same) a.q_out = a.q;
-            else CHECK(operand(e, func, &a.q_out, span(row, a.batch.tokens, a.q_out_token_stride, a.q_heads, a.q_out_head_stride), "q_out", stream));
-            CHECK(operand(e, func, &a.k, span(row, a.batch.tokens, a.k_token_stride, a.kv_heads, a.k_head_stride), "k", stream));
-            CHECK(operand(e, func, &a.v, span(row, a.batch.tokens, a.v_token_stride, a.kv_heads, a.v_head_stride), "v", stream));
-            CHECK(operand(e, func, &a.inv_freq, 4ull * a.rotary_dim, "inv_freq", stream));
-        }
-        return tsw_kv_append(e->cfg.device, &a, stream);
+        const DeviceGuard guard(e->cfg.device);
+        Lock g1(repo().mu);
+        Lock g2(e->mu);
+        CHECK(operand_pages(e, func, a.cache, row, a.kv_heads, stream));
+        CHECK(operand_batch(e, func, a.batch, stream));
+        const bool same = a.q == a.q_out;
+        CHECK(operand(e, func, &a.q, span(row, a.batch.tokens, a.q_token_stride, a.q_heads, a.q_head_stride), "q", stream));
+        if (same) a.q_out = a.q;
+        else CHECK(operand(e, func, &a.q_out, span(row, a.batch.tokens, a.q_out_token_stride, a.q_heads, a.q_out_head_stride), "q_out", stream));
+        CHECK(operand(e, func, &a.k, span(row, a.batch.tokens, a.k_token_stride, a.kv_heads, a.k_head_stride), "k", stream));
+        CHECK(operand(e, func, &a.v, span(row, a.batch.tokens, a.v_token_stride, a.kv_heads, a.v_head_stride), "v", stream));
+        CHECK(operand(e, func, &a.inv_freq, 4ull * a.rotary_dim, "inv_freq", stream));
+        const int rc = tsw_kv_append(e->cfg.device, &a, stream);
+        if (rc == TSW_OK) ++e->kernel_launches;
+        return rc;
     });
 }
 
@@ -316,21 +317,23 @@ int tsw_func_prefix_attention(tsw_engine* e, const char* func, const tsw_prefix_
         CHECK(check_attention(*args));
         tsw_prefix_attention_args a = *args;
         const uint64_t row = 2ull * a.head_dim;
-        {
-            Lock g1(repo().mu);
-            Lock g2(e->mu);
-            CHECK(operand_pages(e, func, a.cache, row, a.kv_heads, stream));
-            if (a.prefix_len) {
-                CHECK(operand_pages(e, func, a.prefix, row, a.kv_heads, stream));
-                const uint64_t n = ((uint64_t)a.prefix_len + a.prefix.page_size - 1) / a.prefix.page_size;
-                CHECK(operand(e, func, &a.prefix_table, 4 * n, "prefix_table", stream));
-            }
-            CHECK(operand_batch(e, func, a.batch, stream));
-            CHECK(operand(e, func, &a.q, span(row, a.batch.tokens, a.q_token_stride, a.q_heads, a.q_head_stride), "q", stream));
-            CHECK(operand(e, func, &a.out, span(row, a.batch.tokens, a.out_token_stride, a.q_heads, a.out_head_stride), "out", stream));
-            CHECK(operand(e, func, &a.lse, 4ull * a.batch.tokens * a.q_heads, "lse", stream));
+        const DeviceGuard guard(e->cfg.device);
+        Lock g1(repo().mu);
+        Lock g2(e->mu);
+        CHECK(operand_pages(e, func, a.cache, row, a.kv_heads, stream));
+        if (a.prefix_len) {
+            CHECK(operand_pages(e, func, a.prefix, row, a.kv_heads, stream));
+            const uint64_t n = ((uint64_t)a.prefix_len + a.prefix.page_size - 1) / a.prefix.page_size;
+            CHECK(operand(e, func, &a.prefix_table, 4 * n, "prefix_table", stream));
         }
-        return tsw_prefix_attention(e->cfg.device, &a, stream);
+        CHECK(operand_batch(e, func, a.batch, stream));
+        CHECK(operand(e, func, &a.q, span(row, a.batch.tokens, a.q_token_stride, a.q_heads, a.q_head_stride), "q", stream));
+        CHECK(operand(e, func, &a.out, span(row, a.batch.tokens, a.out_token_stride, a.q_heads, a.out_head_stride), "out", stream));
+        CHECK(operand(e, func, &a.lse, 4ull * a.batch.tokens * a.q_heads, "lse", stream));
+        CHECK(operand(e, func, &a.workspace, a.workspace_bytes, "workspace", stream));
+        const int rc = tsw_prefix_attention(e->cfg.device, &a, stream);
+        if (rc == TSW_OK) ++e->kernel_launches;
+        return rc;
     });
 }
 

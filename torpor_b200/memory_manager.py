@@ -201,6 +201,23 @@ class MemoryManager:
     def valid_memory_address(self, func: str, ptr: int) -> bool:
         return check(self.L.tsw_valid_memory_address(self.h, func.encode(), ptr)) == 1
 
+    # ---- key/value cache operators on a function's own memory (client addresses throughout)
+    def kv_append(self, func: str, args: "_cabi.KvAppendArgs", stream: int = 0) -> None:
+        """Rotate and append new keys and values (``tsw_func_kv_append``); parameters among the operands that
+        are still being swapped in are waited for on ``stream``, not on the host."""
+        check(self.L.tsw_func_kv_append(self.h, func.encode(), C.byref(args), stream))
+
+    def prefix_attention(self, func: str, args: "_cabi.PrefixAttentionArgs", stream: int = 0) -> None:
+        """Attention behind a shared prefix (``tsw_func_prefix_attention``): the prefix may be among the function's
+        parameters, so that a swap-in brings it along; it is waited for on ``stream``."""
+        check(self.L.tsw_func_prefix_attention(self.h, func.encode(), C.byref(args), stream))
+
+    def prefix_attention_workspace(self, args: "_cabi.PrefixAttentionArgs") -> int:
+        """Bytes of workspace the call needs (``tsw_prefix_attention_workspace``)."""
+        need = C.c_uint64()
+        check(self.L.tsw_prefix_attention_workspace(C.byref(args), C.byref(need)))
+        return need.value
+
     # ---- scenario aliases shared with the checkers
     def track_begin(self, f): self.set_track_model_memory(f)
     def track_end(self, f): self.unset_track_model_memory(f)

@@ -181,6 +181,28 @@ def weight_set(name: str, seed: int | None = None) -> WeightSet:
     return WeightSet(name, default_seed if seed is None else seed, tuple(builder(dtype)))
 
 
+@dataclasses.dataclass(frozen=True)
+class AttentionShape:
+    """What the key/value cache operators need to know of an architecture."""
+    layers: int
+    heads: int
+    kv_heads: int
+    head_dim: int
+
+
+ATTENTION = {"llama_tiny": AttentionShape(2, 8, 8, 128), "llama_mid": AttentionShape(4, 32, 32, 128),
+             "llama2_7b": AttentionShape(32, 32, 32, 128)}
+
+
+def with_prompt(ws: WeightSet, arch: str, tokens: int, page_size: int = 16) -> WeightSet:
+    """``ws`` with the keys and values of the function's own prompt as parameters behind its weights, so that a
+    swap brings them along: per layer two tensors [pages, page_size, kv_heads, head_dim]."""
+    a, dtype = ATTENTION[arch], ws.tensors[0].dtype
+    shape = (-(-tokens // page_size), page_size, a.kv_heads, a.head_dim)
+    extra = [Tensor(f"model.layers.{l}.prompt.{what}", shape, dtype) for l in range(a.layers) for what in ("keys", "values")]
+    return dataclasses.replace(ws, tensors=ws.tensors + tuple(extra))
+
+
 def tensor_values(ws: WeightSet, index: int) -> np.ndarray:
     """Tensor ``index`` of ``ws``: N(0, 0.02) drawn in float32 from the stream
     ``default_rng([seed, index])`` and cast to the set's dtype.  One stream per
