@@ -29,14 +29,31 @@ namespace {
 // of q, k and v do not depend on it and are issued first.
 constexpr int kAppendThreads = 256;
 constexpr int kAppendUnroll = 3;
+constexpr uint64_t kFarBytes = 64ull << 20;      // half of the L2
 
 template <typename V> struct Two { V a, b; };
+
+// Inputs are read once.  What is written is read next by the attention, so it stays in the L2 unless the call writes
+// more than that holds (`far`): then it only drives out what is still to be read.  16384 tokens of 96 heads of
+// 128: 165 us without the hints, 146 with them, 123 at the copy rate.
+template <typename V> __device__ __forceinline__ V load_once(uint64_t p) {
+    V x;
+    if constexpr (sizeof(V) == 16) *(uint4*)&x = __ldcs((const uint4*)p);
+    else x = *(const V*)p;
+    return x;
+}
+template <typename V> __device__ __forceinline__ void store(uint64_t p, const V& x, bool far) {
+    if constexpr (sizeof(V) == 16) {
+        if (far) __stcs((uint4*)p, *(const uint4*)&x);
+        else *(uint4*)p = *(const uint4*)&x;
+    } else *(V*)p = x;
+}
 
 template <typename T, int VEC> struct alignas(VEC * sizeof(T)) Vec { T e[VEC]; };
 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ tsw_kv_append_args a,
-                                                                   uint32_t rows_per_cta) {
+                                                                   uint32_t rows_per_cta, bool far) {
     extern __shared__ float2 s_turn[];            // cos, sin of the token's position for each pair
     __shared__ int s_found[3];                    // own token number, page, place; page < 0: nothing is cached
     const uint32_t tok = blockIdx.x;
@@ -69,10 +86,10 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
         const uint64_t base = c.kind == 0 ? a.q + tok * a.q_token_stride + c.head * a.q_head_stride
                               : c.kind == 1 ? a.k + tok * a.k_token_stride + c.head * a.k_head_stride
                                             : a.v + tok * a.v_token_stride + c.head * a.v_head_stride;
-        x.a = *(const V*)(base + c.oa * sizeof(T));
-        x.b = *(const V*)(base + c.ob * sizeof(T));
+        x.a = load_once<V>(base + c.oa * sizeof(T));
+        x.b = load_once<V>(base + c.ob * sizeof(T));
     };
-    auto store = [&](const Unit& c, Two<V>& x) {
+    auto finish = [&](const Unit& c, Two<V>& x) {
         uint64_t base;
         if (c.kind == 0) base = a.q_out + tok * a.q_out_token_stride + c.head * a.q_out_head_stride;
         else if (s_found[1] < 0) return;
@@ -109,8 +126,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
                 }
             }
         }
-        *(V*)(base + c.oa * sizeof(T)) = x.a;
-        *(V*)(base + c.ob * sizeof(T)) = x.b;
+        store(base + c.oa * sizeof(T), x.a, far);
+        store(base + c.ob * sizeof(T), x.b, far);
     };
 
     Two<V> x[kAppendUnroll];
@@ -154,12 +171,12 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
 #pragma unroll
     for (int u = 0; u < kAppendUnroll; ++u) {
         const uint32_t i = threadIdx.x + u * kAppendThreads;
-        if (i < n) store(cut(i), x[u]);
+        if (i < n) finish(cut(i), x[u]);
     }
     for (uint32_t i = threadIdx.x + kAppendUnroll * kAppendThreads; i < n; i += kAppendThreads) {
         const Unit c = cut(i);
         load(c, x[0]);
-        store(c, x[0]);
+        finish(c, x[0]);
     }
 }
 
@@ -254,17 +271,17 @@ cudaError_t launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t sme
 }
 
 template <typename T, int VEC>
-cudaError_t launch_append(const tsw_kv_append_args& a, dim3 grid, uint32_t rows_per_cta, cudaStream_t stream) {
-    return launch(kv_append_kernel<T, VEC>, grid, kAppendThreads, sizeof(float2) * (a.rotary_dim / 2), stream, a, rows_per_cta);
+cudaError_t launch_append(const tsw_kv_append_args& a, dim3 grid, uint32_t rows_per_cta, bool far, cudaStream_t stream) {
+    return launch(kv_append_kernel<T, VEC>, grid, kAppendThreads, sizeof(float2) * (a.rotary_dim / 2), stream, a, rows_per_cta, far);
 }
 
 template <typename T>
-cudaError_t launch_append_vec(const tsw_kv_append_args& a, int vec, dim3 grid, uint32_t rows_per_cta, cudaStream_t stream) {
+cudaError_t launch_append_vec(const tsw_kv_append_args& a, int vec, dim3 grid, uint32_t rows_per_cta, bool far, cudaStream_t stream) {
     switch (vec) {
-        case 8: return launch_append<T, 8>(a, grid, rows_per_cta, stream);
-        case 4: return launch_append<T, 4>(a, grid, rows_per_cta, stream);
-        case 2: return launch_append<T, 2>(a, grid, rows_per_cta, stream);
-        default: return launch_append<T, 1>(a, grid, rows_per_cta, stream);
+        case 8: return launch_append<T, 8>(a, grid, rows_per_cta, far, stream);
+        case 4: return launch_append<T, 4>(a, grid, rows_per_cta, far, stream);
+        case 2: return launch_append<T, 2>(a, grid, rows_per_cta, far, stream);
+        default: return launch_append<T, 1>(a, grid, rows_per_cta, far, stream);
     }
 }
 
@@ -285,8 +302,9 @@ cudaError_t launch_kv_append(const tsw_kv_append_args& a, int device_sms, cudaSt
     const uint32_t groups = std::max(1u, std::min((rows + 7) / 8, (uint32_t)(2 * device_sms) / std::max(1u, a.batch.tokens)));
     const uint32_t rows_per_cta = (rows + groups - 1) / groups;
     const dim3 grid(a.batch.tokens, (rows + rows_per_cta - 1) / rows_per_cta);
-    return a.dtype == TSW_F16 ? launch_append_vec<__half>(a, vec, grid, rows_per_cta, stream)
-                              : launch_append_vec<__nv_bfloat16>(a, vec, grid, rows_per_cta, stream);
+    const bool far = 2ull * rows * a.batch.tokens * a.head_dim > kFarBytes;
+    return a.dtype == TSW_F16 ? launch_append_vec<__half>(a, vec, grid, rows_per_cta, far, stream)
+                              : launch_append_vec<__nv_bfloat16>(a, vec, grid, rows_per_cta, far, stream);
 }
 
 cudaError_t launch_prefix_attention_rows(const tsw_prefix_attention_args& a, cudaStream_t stream) {
