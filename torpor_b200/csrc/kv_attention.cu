@@ -722,13 +722,14 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(const __grid_cons
     read_rows(a.batch, b, a.max_q, a.cache.page_size, r);
     if (tok >= r.first + r.n) return;
     uint32_t before = 0;
-    for (int rt = (tok - r.first) / own_item_tokens(d), i = lane; i < rt; i += 32) {
+#pragma unroll 1
+    for (int rt = (int)((uint32_t)(tok - r.first) / (uint32_t)own_item_tokens(d)), i = lane; i < rt; i += 32) {
         const Cut c = cut_own(d, r, i);
         before += max(c.kt_a, c.kt_b);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(~0u, before, o);
-    const int kv_head = min(head, (int)a.q_heads - 1) / w.group;
+    const uint32_t kv_head = min((uint32_t)head, a.q_heads - 1) / w.group;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint8_t* ws = (const uint8_t*)a.workspace;
     const uint32_t* base = (const uint32_t*)(ws + w.own_base);
@@ -744,7 +745,7 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(const __grid_cons
     most = max(most, __shfl_xor_sync(~0u, most, 16));
     const uint64_t row = (uint64_t)tok * a.q_heads + head;
     // The i-th part: of the prefix list first, in each list the one by row, then those of the ranges that continue.
-    const uint32_t in_group = head % w.group;
+    const uint32_t in_group = head - kv_head * w.group;
     const uint64_t home0 = home_index(d, 0, row, a.q_heads), home1 = home_index(d, 1, row, a.q_heads);
     auto part = [&](int i) -> uint64_t {             // its place; bit 63: among those of the ranges that continue
         const bool l = i >= n0;
@@ -757,6 +758,7 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(const __grid_cons
     float4 acc[kVec];
 #pragma unroll
     for (int e = 0; e < kVec; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
     for (int i0 = 0; i0 < most; i0 += 8) {
         float2 mine = make_float2(-INFINITY, 0.f);
         uint64_t at = 0;
@@ -768,7 +770,7 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(const __grid_cons
 #pragma unroll
         for (int o = 4; o; o >>= 1) next = fmaxf(next, __shfl_xor_sync(~0u, next, o));
         const float base_m = next == -INFINITY ? 0.f : next;
-        const float keep = exp2f(top - base_m), f = mine.x == -INFINITY && mine.y == 0.f ? 0.f : exp2f(mine.x - base_m);
+        const float keep = exp2_fast(top - base_m), f = mine.x == -INFINITY && mine.y == 0.f ? 0.f : exp2_fast(mine.x - base_m);
         float add = mine.y * f;
 #pragma unroll
         for (int o = 4; o; o >>= 1) add += __shfl_xor_sync(~0u, add, o);
@@ -782,7 +784,7 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(const __grid_cons
             acc[e].w *= keep;
         }
         const int m = min(8, most - i0);
-#pragma unroll 2
+#pragma unroll 4
         for (int i = 0; i < m; ++i) {
             const float fi = __shfl_sync(~0u, f, (lane & 24) + i);
             const uint64_t from = __shfl_sync(~0u, at, (lane & 24) + i);

@@ -17,6 +17,12 @@
 #define TSW_HD_CALL
 #endif
 
+#ifdef __CUDA_ARCH__
+#define TSW_ROLLED _Pragma("unroll 1")
+#else
+#define TSW_ROLLED
+#endif
+
 namespace tsw {
 
 constexpr int kTile = 128;                    // keys in a step, rows in a tile
@@ -111,7 +117,7 @@ struct Deal {                  // what the dealing depends on
 
 // An item of the own list: some rows of one sequence (one row tile, or two when dealt in pairs) and a key head.
 struct Cut { int tok, n_a, n_b, kt_a, kt_b; };     // first token, tokens of the two row tiles, key tiles each sees
-TSW_HD int tiles_of(int keys) { return (keys + kTile - 1) / kTile; }
+TSW_HD int tiles_of(int keys) { return (int)((uint32_t)(keys + kTile - 1) / kTile); }     // keys >= 0
 TSW_HD int own_item_tokens(const Deal& d) { return d.w.own_pair ? 2 * d.w.tile_tokens : d.w.tile_tokens; }
 TSW_HD int prefix_item_tokens(const Deal& d) { return d.w.prefix_pair ? 2 * d.w.tile_tokens : d.w.tile_tokens; }
 TSW_HD Cut cut_own(const Deal& d, const SeqRows& r, int rt) {
@@ -127,6 +133,7 @@ TSW_HD Cut cut_own(const Deal& d, const SeqRows& r, int rt) {
 }
 TSW_HD_CALL inline uint32_t sequence_tiles(const Deal& d, const SeqRows& r) {     // over all key heads
     uint32_t sum = 0;
+    TSW_ROLLED
     for (int rt = 0, per = own_item_tokens(d); rt * per < r.n; ++rt) {
         const Cut c = cut_own(d, r, rt);
         sum += imax(c.kt_a, c.kt_b);
@@ -137,7 +144,7 @@ TSW_HD_CALL inline uint32_t sequence_tiles(const Deal& d, const SeqRows& r) {   
 // A list of `total` tiles is cut into n ranges, none of them empty; range i starts at i * total / n.  The range that
 // holds tile x; how many there are; the range of a CTA's stream (neighbours on different CTAs, so that few ranges
 // spread over many); the streams' places for partial results, numbered by range.
-TSW_HD_CALL inline uint32_t quotient(uint64_t a, uint32_t b) { return (uint32_t)(a / b); }
+TSW_HD_CALL inline uint32_t quotient(uint64_t a, uint32_t b) { return a >> 32 ? (uint32_t)(a / b) : (uint32_t)a / b; }      // 32 bits are the quick way
 TSW_HD uint32_t range_start(uint32_t i, uint32_t total, uint32_t n) { return quotient((uint64_t)i * total, n); }
 TSW_HD uint32_t range_of(uint32_t x, uint32_t total, uint32_t n) { return quotient(((uint64_t)x + 1) * n - 1, total); }
 TSW_HD uint32_t ranges(const Deal& d, bool pair, uint32_t total) {
@@ -177,14 +184,16 @@ TSW_HD uint32_t prefix_rows(const Deal& d, int& tok0, int& tok1) {      // row t
     const int* cu = (const int*)d.batch.cu_q;
     tok0 = imin(imax(cu[0], 0), (int)d.batch.tokens);
     tok1 = imin(imax(cu[d.batch.batch], tok0), (int)d.batch.tokens);
-    const int per = prefix_item_tokens(d);
-    return (uint32_t)((tok1 - tok0 + per - 1) / per);
+    const uint32_t per = prefix_item_tokens(d);
+    return (tok1 - tok0 + per - 1) / per;
 }
 // Tile `off` of the own tiles of sequences [lo, hi) begins a range of `left` tiles.
 TSW_HD_CALL inline bool find_start(const Deal& d, int lo, int hi, uint32_t off, uint32_t left, Start& s) {
+    TSW_ROLLED
     for (int b = lo; b < hi; ++b) {
         SeqRows r;
         read_rows(d.batch, b, d.max_q, d.page_size, r);
+        TSW_ROLLED
         for (int rt = 0, per = own_item_tokens(d); rt * per < r.n; ++rt) {
             const Cut c = cut_own(d, r, rt);
             const uint32_t n = imax(c.kt_a, c.kt_b), all = n * d.kv_heads;
@@ -374,26 +383,27 @@ TSW_HD RowJob make_row_job(const Deal& d, const Job& j, bool pair, int s, uint32
 // Where the partial results of one row lie: of each list the ranges first .. last, its half of a pair and its
 // token's place in the row tile.  `before`: own tiles of the row's sequence in front of its item (one head).
 struct Parts { bool has; uint32_t first, last, half, place; };
+TSW_HD uint32_t split_rows(const Deal& d, bool pair, uint32_t at, Parts& p) {      // the item of row token `at` of a list
+    const uint32_t tile = at / d.w.tile_tokens;
+    p.place = at - tile * d.w.tile_tokens;
+    p.half = pair ? tile & 1 : 0;
+    return pair ? tile >> 1 : tile;
+}
 TSW_HD Parts prefix_parts(const Deal& d, int tok, int kv_head, uint32_t total) {
     Parts p = {};
     int tok0, tok1;
     const uint32_t rts = prefix_rows(d, tok0, tok1);
     if (!total || tok < tok0 || tok >= tok1) return p;
-    const int per = prefix_item_tokens(d), at = tok - tok0;
-    const uint32_t x = (kv_head * rts + at / per) * d.w.prefix_tiles, n = ranges(d, d.w.prefix_pair, total);
+    const uint32_t item = split_rows(d, d.w.prefix_pair, tok - tok0, p), x = (kv_head * rts + item) * d.w.prefix_tiles;
+    const uint32_t n = ranges(d, d.w.prefix_pair, total);
     p.has = true;
     p.first = range_of(x, total, n);
     p.last = range_of(x + d.w.prefix_tiles - 1, total, n);
-    p.half = (at % per) / d.w.tile_tokens;
-    p.place = at % d.w.tile_tokens;
     return p;
 }
 TSW_HD Parts own_parts(const Deal& d, const SeqRows& r, int tok, int kv_head, uint32_t base, uint32_t before, uint32_t total) {
     Parts p = {};
-    const int per = own_item_tokens(d), at = tok - r.first;
-    const Cut c = cut_own(d, r, at / per);
-    p.half = (at % per) / d.w.tile_tokens;
-    p.place = at % d.w.tile_tokens;
+    const Cut c = cut_own(d, r, split_rows(d, d.w.own_pair, tok - r.first, p));
     const int seen = p.half ? c.kt_b : c.kt_a;
     if (!seen) return p;
     const uint32_t x = base + before * d.kv_heads + kv_head * imax(c.kt_a, c.kt_b), n = ranges(d, d.w.own_pair, total);

@@ -35,6 +35,7 @@ __device__ __forceinline__ float warp_sum(float x) {
 __device__ __forceinline__ int find_sequence(const int* cu_q, uint32_t batch, uint32_t tok) {
     const int lane = threadIdx.x & 31;
     uint32_t lo = 0, hi = batch + 1;              // entries [0, lo) are <= tok (lo >= 1 once any is), [hi, ..) are > tok
+#pragma unroll 1
     while (lo < hi) {
         const uint32_t span = hi - lo, step = (span + 31) / 32;
         const uint32_t at = lo + lane * step;     // first entry of this lane's piece
