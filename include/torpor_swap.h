@@ -393,7 +393,7 @@ typedef struct {
     tsw_kv_pages prefix;                 /* where the prefix pages lie; often equal to cache */
     tsw_kv_batch batch;
     uint64_t prefix_table;               /* int32 [ceil(prefix_len / prefix.page_size)] in device memory */
-    uint64_t q, out;                     /* [tokens][q_heads][head_dim] */
+    uint64_t q, out;                     /* [tokens][q_heads][head_dim], apart from one another */
     uint64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
     uint64_t lse;                        /* optional (0) */
     uint64_t workspace, workspace_bytes;

@@ -127,7 +127,8 @@ def test_tables_out_of_order_are_recorded_not_followed():
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("q_heads,kv_heads,dim,page_size,head_major", [
     (4, 4, 64, 16, False), (8, 2, 128, 16, True), (28, 4, 128, 64, False), (7, 1, 96, 8, False), (16, 1, 80, 32, True),
-    (3, 3, 128, 256, False), (32, 8, 64, 128, True), (5, 5, 40, 16, False), (2, 1, 72, 1, False)])
+    (3, 3, 128, 256, False), (32, 8, 64, 128, True), (5, 5, 40, 16, False), (2, 1, 72, 1, False), (2, 1, 8, 16, False), (6, 2, 120, 32, True),
+    (128, 1, 64, 16, False), (96, 1, 128, 64, False), (130, 1, 64, 16, False), (4, 4, 256, 16, False), (4, 2, 50, 24, False)])
 def test_attention_heads_and_pages(dtype, q_heads, kv_heads, dim, page_size, head_major):
     c = Batch([1, 1, 1, 1], [1, 37, 128, 300], q_heads=q_heads, kv_heads=kv_heads, dim=dim, page_size=page_size, head_major=head_major,
               dtype=dtype, prefix=150, seed=q_heads + dim)
@@ -146,6 +147,16 @@ def test_attention_lengths_and_masks(prefix, q_lens, own, causal):
     c.check(out, lse, causal=causal)
     _, _, _, _, own_rows = c.attend(causal=causal)
     assert (out[~own_rows] == 5.0).all(), "rows of nobody were written"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_more_sequences_than_threads(dtype):
+    """Every CTA sums all sequences' tiles: some thread has several, many have none; empty sequences among them."""
+    n = 900
+    c = Batch([(i * 5) % 2 for i in range(n)], [(i * 7) % 9 for i in range(n)], q_heads=2, kv_heads=1, dim=64, prefix=40, page_size=8, dtype=dtype,
+              seed=19)
+    out, lse = attend(c, return_lse=True)
+    c.check(out, lse)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -342,6 +353,47 @@ def test_captured_steps_follow_the_tables():
             ref = step()
             assert torch.equal(out, ref[1])
             c.check(out, q=q)
+
+
+def test_whole_path_on_another_stream():
+    """Tables, inputs and calls on a stream of the caller's, nothing on the default one."""
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        c = Batch([1, 30, 1], [200, 30, 77], prefix=140, dim=128, q_heads=8, kv_heads=2, seed=43)
+        q = kv_cache.kv_append(c.k_cache, c.v_cache, c.k, c.v, c.table, c.lens, c.cu_q, inv_freq=kv_cache.rope_frequencies(128),
+                               position_offset=140, q=c.q)
+        out, lse = kv_cache.prefix_attention(q, c.k_cache, c.v_cache, c.table, c.lens, c.cu_q, max_q=30, prefix_table=c.prefix_table,
+                                             prefix_len=140, return_lse=True)
+    side.synchronize()
+    c.check(out, lse, q=q)
+
+
+def test_given_workspace():
+    c = Batch([1] * 5, [300 + i for i in range(5)], prefix=700, dim=128, q_heads=8, kv_heads=2, seed=44)
+    want = attend(c)
+    for size, ok in ((64 << 20, True), (256, False)):
+        ws = torch.full((size,), 0xFF, dtype=torch.uint8, device="cuda")
+        if ok:
+            assert torch.equal(attend(c, workspace=ws), want)        # whatever it holds
+            assert torch.equal(attend(c, workspace=ws), want)
+            with pytest.raises(SwapError):
+                attend(c, workspace=ws[64:])                          # not 256-byte aligned
+        else:
+            with pytest.raises(ValueError):
+                attend(c, workspace=ws)
+
+
+def test_not_a_number_in_a_visible_key_shows():
+    """Nothing is swept under: a NaN or an infinity among the keys or values a row sees leaves that row not finite,
+    and rows of other sequences as they were."""
+    for what in ("k_cache", "v_cache"):
+        for bad in (math.nan, math.inf):
+            c = Batch([1, 1, 1], [200, 190, 77], prefix=140, dim=64, seed=45)
+            good = attend(c)
+            getattr(c, what)[int(c.table[1, 3]), 5] = bad
+            out = attend(c)
+            assert torch.equal(out[0], good[0]) and torch.equal(out[2], good[2])
+            assert not torch.isfinite(out[1]).all()
 
 
 def test_calls_on_two_streams_at_once():

@@ -86,13 +86,13 @@ APPEND_REFUSED = [
     dict(position_offset=1 << 32), dict(k_token_stride=1 << 41), dict(cache__page_size=0), dict(cache__page_size=1 << 21), dict(cache__k=0),
     dict(cache__k_head_stride=0), dict(cache__v_token_stride=64), dict(cache__k_page_stride=2), dict(cache__v=(1 << 41) + 1),
     dict(batch__seq_lens=0), dict(batch__cu_q=0), dict(batch__page_table=0), dict(batch__table_stride=3), dict(batch__page_table=4098),
-    dict(batch__tokens=1 << 31), dict(batch__batch=1 << 24), dict(q_out=1 << 42, q_out_head_stride=256, q_out_token_stride=1024),
+    dict(batch__tokens=1 << 31), dict(batch__tokens=(1 << 28) + 1), dict(batch__batch=1 << 24), dict(q_out=1 << 42, q_out_head_stride=256, q_out_token_stride=1024),
 ]
 ATTENTION_REFUSED = [
     dict(dtype=2), dict(head_dim=0), dict(head_dim=513), dict(q_heads=0), dict(q_heads=5), dict(kv_heads=0), dict(q=0), dict(out=0),
     dict(out_head_stride=64), dict(out_token_stride=0), dict(out=(1 << 43) + 1), dict(scale=float("nan")), dict(scale=float("inf")),
     dict(prefix_table=0), dict(prefix_table=2), dict(prefix_len=0x7fffff01), dict(prefix__k=0), dict(prefix__page_size=0), dict(lse=2),
-    dict(max_q=1 << 31), dict(cache__v=0), dict(cache__k_page_stride=1 << 41), dict(batch__cu_q=0), dict(batch__table_stride=2),
+    dict(max_q=1 << 31), dict(out=1 << 42), dict(batch__tokens=(1 << 28) + 1), dict(batch__tokens=1 << 28, q_heads=64), dict(cache__v=0), dict(cache__k_page_stride=1 << 41), dict(batch__cu_q=0), dict(batch__table_stride=2),
 ]
 
 

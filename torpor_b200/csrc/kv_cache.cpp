@@ -72,7 +72,7 @@ int check_pages(const tsw_kv_pages& p, uint64_t row_bytes, uint32_t heads, bool 
 }
 
 int check_batch(const tsw_kv_batch& b) {
-    if (b.tokens > 0x7fffffffu || b.batch > 0xffffffu) return bad("tokens or batch out of range");
+    if (b.tokens > 1u << 28 || b.batch > 0xffffffu) return bad("tokens or batch out of range");
     if (b.batch && (!b.seq_lens || !b.cu_q)) return bad("seq_lens and cu_q must be given");
     if (b.table_width && !b.page_table) return bad("page_table is null");
     if (b.batch > 1 && b.table_stride < b.table_width) return bad("table_stride is smaller than table_width");
@@ -140,6 +140,8 @@ int check_attention(const tsw_prefix_attention_args& a) {
     if (a.max_q > 0x7fffffffu) return bad("max_q out of range");
     if (!(a.scale == a.scale) || a.scale - a.scale != 0.f) return bad("scale must be finite");
     if (a.lse & 3) return bad("lse must be 4-byte aligned");
+    if ((uint64_t)a.batch.tokens * a.q_heads >> 32) return bad("too many rows for one call");
+    if (a.batch.tokens && a.out == a.q) return bad("out must not be q");
     CHECK(check_rows("q", a.q, a.q_token_stride, a.q_head_stride, a.batch, a.q_heads, row, false));
     return check_rows("out", a.out, a.out_token_stride, a.out_head_stride, a.batch, a.q_heads, row, true);
 }

@@ -117,7 +117,7 @@ struct Deal {                  // what the dealing depends on
 
 // An item of the own list: some rows of one sequence (one row tile, or two when dealt in pairs) and a key head.
 struct Cut { int tok, n_a, n_b, kt_a, kt_b; };     // first token, tokens of the two row tiles, key tiles each sees
-TSW_HD int tiles_of(int keys) { return (int)((uint32_t)(keys + kTile - 1) / kTile); }     // keys >= 0
+TSW_HD int tiles_of(int keys) { return (int)(((uint32_t)keys + kTile - 1) / kTile); }     // keys >= 0
 TSW_HD int own_item_tokens(const Deal& d) { return d.w.own_pair ? 2 * d.w.tile_tokens : d.w.tile_tokens; }
 TSW_HD int prefix_item_tokens(const Deal& d) { return d.w.prefix_pair ? 2 * d.w.tile_tokens : d.w.tile_tokens; }
 TSW_HD Cut cut_own(const Deal& d, const SeqRows& r, int rt) {
