@@ -283,31 +283,42 @@ struct Walk {
     Cursor c0, c1;
     Job j0, j1;
     int kt0 = 0, kt1 = 0;
-    bool live0 = false, live1 = false, last = true, own = false, pair = false;
-    TSW_HD Walk(const Deal& d, const Prologue& pro) : c0(pro, 0), c1(pro, 1) { begin(d, pro); }
-    TSW_HD void pull0(const Deal& d, const Prologue& pro) {
-        live0 = c0.next(d, pro, own, j0);
-        kt0 = j0.kt0;
-    }
-    TSW_HD void pull1(const Deal& d, const Prologue& pro) {
-        live1 = c1.next(d, pro, own, j1);
-        kt1 = j1.kt0;
-    }
-    TSW_HD void begin(const Deal& d, const Prologue& pro) {
-        pair = own ? d.w.own_pair : d.w.prefix_pair;
-        last = true;
-        pull0(d, pro);
-        live1 = false;
-        if (!pair) pull1(d, pro);
+    bool live0 = false, live1 = false, need0 = true, need1, last = true, own = false, pair;
+    TSW_HD Walk(const Deal& d, const Prologue& pro) : c0(pro, 0), c1(pro, 1) {
+        pair = d.w.prefix_pair;
+        need1 = !pair;
     }
     // The next tile: its job, its number, and which streams have a product with it.  False at the end.
     TSW_HD bool next(const Deal& d, const Prologue& pro, Job& j, int& tile, bool& use0, bool& use1) {
-        if (!last && live0 && kt0 == j0.kt1) pull0(d, pro);
-        if (last && live1 && kt1 == j1.kt1) pull1(d, pro);
-        while (!live0 && !live1) {
+        need0 = need0 || (!last && live0 && kt0 == j0.kt1);
+        need1 = need1 || (last && live1 && kt1 == j1.kt1);
+        TSW_ROLLED
+        for (;;) {
+            if (need0 || need1) {               // one copy of the search for both cursors
+                Cursor c = need0 ? c0 : c1;
+                const bool live = c.next(d, pro, own, j);
+                if (need0) {
+                    c0 = c;
+                    j0 = j;
+                    live0 = live;
+                    kt0 = live ? j.kt0 : 0;
+                    need0 = false;
+                } else {
+                    c1 = c;
+                    j1 = j;
+                    live1 = live;
+                    kt1 = live ? j.kt0 : 0;
+                    need1 = false;
+                }
+                continue;
+            }
+            if (live0 || live1) break;
             if (own) return false;
             own = true;
-            begin(d, pro);
+            pair = d.w.own_pair;
+            last = true;
+            need0 = true;
+            need1 = !pair;
         }
         last = last ? !live0 : live1;
         if (last) {
