@@ -484,9 +484,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
                 for (int h = 0; h < halves; ++h) {
                     const int mine = min(kHalf, keys - h * kHalf);
                     const bool tail = mine & 15;                  // the rows will clear what lies behind: the values have to be there
-                    if (tail) {
-                        if (held_steps) product_o();
-                        if (!ok || (h == 0 && !see_v(v_slot(u), pair))) break;
+                    if (tail && (h == 0 || (held_steps && held_wait))) {       // else the O product of the lower half has seen them
+                        const uint32_t y = (pair ? 0 : s * S::kV) + v_slot(u);
+                        if (held_steps && !mbar_test(bar + B::v_full + 8 * y, v_ph >> y & 1)) product_o();
+                        if (ok && (h == 0 || held_steps)) {
+                            see_v(v_slot(u), pair);
+                            if (h) held_wait = false;
+                        }
+                        if (!ok) break;
                     }
                     const uint32_t k_lo = desc_lo(k_at + slot * S::kTileBytes + h * kHalf * 128, 16), t_x = t_s + (n & 1) * kHalf;
                     fence_after();
