@@ -19,7 +19,7 @@
 // loads run under the other's exponentials.  The streams take different items (few rows: bound by HBM), or two row
 // tiles of one item that share every key tile ("pair": many rows, where a load of 64 KB per 128 rows and tile would
 // ask 128 bytes a cycle of the L2).  A stream's S is two buffers of 64 keys: with one of 128 its rows waited 2000
-// of 4100 cycles a tile for O and the next S; now there is always one to work on.  Six warps do the rest: one
+// of 4100 cycles a tile for O and the next S; now there is always one to work on.  Five warps do the rest: one
 // thread schedules (units and jobs go to the others through rings in shared memory, so that the lists'
 // arithmetic is done and fetched once), two warps load keys and values page by page with TMA, two
 // threads issue the products.
