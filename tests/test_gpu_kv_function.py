@@ -128,6 +128,21 @@ def test_operands_have_to_be_the_functions(function):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("call,side", [("kv_append", "cache"), ("prefix_attention", "cache"), ("prefix_attention", "prefix")])
+@pytest.mark.parametrize("field", ["k_page_stride", "v_page_stride"])
+def test_pages_that_pass_64_bits_leave_their_block(function, call, side, field):
+    """2^25 strides of 2^39 bytes are 0 modulo 2^64: no reason to take them for a short operand."""
+    eng, decode, model, block, _ = function
+    at = {t.name: model.tensor_vaddr[i] for i, t in enumerate(model.ws.tensors) if ".prompt." in t.name}
+    args = decode._append(block, 0, 0) if call == "kv_append" else decode._attention(block, lambda l, what: at[f"model.layers.{l}.prompt.{what}"], 0, 0)
+    pages = getattr(args, side)
+    pages.pages = (1 << 25) + 1
+    setattr(pages, field, 1 << 39)
+    with pytest.raises(SwapError) as e:
+        getattr(eng, call)("f", args)
+    assert e.value.code == _cabi.ERR_NOT_FOUND, e.value
+
+
 def test_request_stream_with_decoding_functions(built):
     repo_reset()
     out = serving.run_stream(n_gpus=1, n_models=4, rate=40.0, duration_s=1.0, cap_bytes=300 << 20, seed=4, archs=("llama_tiny",),

@@ -192,10 +192,13 @@ int operand(tsw_engine* e, const char* func, uint64_t* addr, uint64_t bytes, con
     return fail(TSW_ERR_NOT_FOUND, std::string(name) + " is not inside any block of the function");
 }
 
-// Bytes from the first to the last element of a strided operand.
+// Bytes from the first to the last element of a strided operand.  Counts of 2^31 and strides of 2^40 are legal each and
+// together pass 64 bits: what does is longer than any block.
 uint64_t span(uint64_t row_bytes, uint64_t n0, uint64_t s0, uint64_t n1, uint64_t s1, uint64_t n2 = 1, uint64_t s2 = 0) {
+    using Wide = unsigned __int128;
     if (!n0 || !n1 || !n2) return 0;
-    return row_bytes + (n0 - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2;
+    const Wide all = row_bytes + Wide(n0 - 1) * s0 + Wide(n1 - 1) * s1 + Wide(n2 - 1) * s2;
+    return all >> 64 ? UINT64_MAX : (uint64_t)all;
 }
 
 int operand_pages(tsw_engine* e, const char* func, tsw_kv_pages& p, uint64_t row, uint32_t heads, void* stream) {
