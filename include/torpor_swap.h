@@ -331,7 +331,8 @@ int tsw_place_segments_static_status(int device, void* stream, uint32_t* status,
  *
  * Types: TSW_F16 and TSW_BF16, the same for all operands of a call; sums, statistics and
  * rotations are held in 32 bits or more, and each result is rounded once.  Strides are in bytes;
- * the elements of a head are contiguous.  Head h of the queries reads key head
+ * the elements of a head are contiguous.  Operands that are written keep their rows apart: taken by stride, each
+ * dimension steps over all that the ones before it cover (TSW_ERR_INVALID otherwise).  Head h of the queries reads key head
  * h / (q_heads / kv_heads).
  *
  * The calls take a device ordinal and a cudaStream_t of that device, allocate nothing, wait for nothing

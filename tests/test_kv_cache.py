@@ -111,6 +111,38 @@ def test_attention_refuses(built, wrong):
     assert L.tsw_prefix_attention_workspace(C.byref(attention_args(**wrong)), C.byref(need)) == _cabi.ERR_INVALID
 
 
+# Each stride alone steps over a row, together they do not.
+OVERLAPPING = [
+    ("append", dict(q_out_token_stride=128)), ("append", dict(q_out_token_stride=256)), ("append", dict(q_out_head_stride=640)),
+    ("append", dict(cache__k_token_stride=128)), ("append", dict(cache__v_head_stride=256)), ("append", dict(cache__k_page_stride=256)),
+    ("append", dict(cache__v_page_stride=15 * 256 + 128)), ("append", dict(cache__k=1 << 41)),
+    ("attend", dict(out_token_stride=128)), ("attend", dict(out_token_stride=384)), ("attend", dict(out_head_stride=256)),
+]
+
+
+@pytest.mark.parametrize("call,wrong", OVERLAPPING, ids=lambda w: w if isinstance(w, str) else "-".join(f"{k}={v}" for k, v in w.items()))
+def test_overlapping_results_are_refused(built, call, wrong):
+    L = _cabi.lib()
+    if call == "append":
+        assert L.tsw_kv_append(0, C.byref(append_args(**wrong)), None) == _cabi.ERR_INVALID
+    else:
+        assert L.tsw_prefix_attention(0, C.byref(attention_args(**wrong)), None) == _cabi.ERR_INVALID
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2), (0, 2, 1), (1, 0, 2), (1, 2, 0), (2, 0, 1), (2, 1, 0)])
+@pytest.mark.parametrize("pad", [0, 16])
+def test_layouts_with_dimensions_in_any_order_are_taken(built, order, pad):
+    """Refused for want of a device at most, and not at all without rows."""
+    a, counts, strides, covered = append_args(batch__tokens=0), (8, 16, 2), [0, 0, 0], 128
+    for d in order:
+        strides[d] = covered + pad
+        covered += (counts[d] - 1) * strides[d]
+    for side in "kv":
+        for d, name in enumerate(("page", "token", "head")):
+            setattr(a.cache, f"{side}_{name}_stride", strides[d])
+    assert _cabi.lib().tsw_kv_append(0, C.byref(a), None) == 0
+
+
 @pytest.mark.parametrize("device", [-1, 64, 1 << 30])
 def test_device_ordinals_out_of_range(built, device):
     L = _cabi.lib()

@@ -3,6 +3,7 @@
 
 #include "engine_internal.hpp"
 
+#include <algorithm>
 #include <atomic>
 
 #include "kv_kernels.hpp"
@@ -52,8 +53,20 @@ int status_word(int device, uint32_t** word) {
 
 int bad(const char* what) { return fail(TSW_ERR_INVALID, what); }
 
-// Does a row of `count` pieces of `bytes` each, `stride` apart, keep the pieces apart?
-bool apart(uint64_t stride, uint64_t count, uint64_t bytes) { return count <= 1 || stride >= bytes; }
+// Are the rows of an operand that is written apart?  Taken by stride, each dimension has to step over all that the
+// ones before it cover; a dimension of one entry steps nowhere.
+struct Steps { uint64_t stride, count; };
+bool apart(uint64_t row_bytes, Steps x, Steps y, Steps z = {0, 1}) {
+    Steps by[3] = {x, y, z};
+    std::sort(by, by + 3, [](const Steps& l, const Steps& r) { return l.stride < r.stride; });
+    unsigned __int128 covered = row_bytes;
+    for (const Steps& s : by) {
+        if (s.count <= 1) continue;
+        if (s.stride < covered) return false;
+        covered += (unsigned __int128)(s.count - 1) * s.stride;
+    }
+    return true;
+}
 
 int check_pages(const tsw_kv_pages& p, uint64_t row_bytes, uint32_t heads, bool written, const char* name) {
     const std::string n(name);
@@ -64,10 +77,10 @@ int check_pages(const tsw_kv_pages& p, uint64_t row_bytes, uint32_t heads, bool 
         return fail(TSW_ERR_INVALID, n + ": addresses and strides must be multiples of the element size");
     for (uint64_t s : {p.k_page_stride, p.k_token_stride, p.k_head_stride, p.v_page_stride, p.v_token_stride, p.v_head_stride})
         if (s >> 40) return fail(TSW_ERR_INVALID, n + ": stride out of range");
-    if (written && !(apart(p.k_page_stride, p.pages, row_bytes) && apart(p.k_token_stride, p.page_size, row_bytes) &&
-                     apart(p.k_head_stride, heads, row_bytes) && apart(p.v_page_stride, p.pages, row_bytes) &&
-                     apart(p.v_token_stride, p.page_size, row_bytes) && apart(p.v_head_stride, heads, row_bytes)))
+    if (written && !(apart(row_bytes, {p.k_page_stride, p.pages}, {p.k_token_stride, p.page_size}, {p.k_head_stride, heads}) &&
+                     apart(row_bytes, {p.v_page_stride, p.pages}, {p.v_token_stride, p.page_size}, {p.v_head_stride, heads})))
         return fail(TSW_ERR_INVALID, n + ": strides make heads, tokens or pages overlap");
+    if (written && p.pages && p.k == p.v) return fail(TSW_ERR_INVALID, n + ": keys and values are the same memory");
     return TSW_OK;
 }
 
@@ -94,7 +107,7 @@ int check_rows(const char* name, uint64_t addr, uint64_t tok, uint64_t head, con
     if (b.tokens && heads && !addr) return fail(TSW_ERR_INVALID, n + " is null");
     if ((addr | tok | head) & 1) return fail(TSW_ERR_INVALID, n + ": address and strides must be multiples of the element size");
     if ((tok >> 40) || (head >> 40)) return fail(TSW_ERR_INVALID, n + ": stride out of range");
-    if (written && !(apart(tok, b.tokens, row_bytes) && apart(head, heads, row_bytes)))
+    if (written && !apart(row_bytes, {tok, b.tokens}, {head, heads}))
         return fail(TSW_ERR_INVALID, n + ": strides make heads or tokens overlap");
     return TSW_OK;
 }
