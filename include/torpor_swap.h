@@ -355,7 +355,7 @@ typedef struct {
     uint64_t seq_lens;      /* int32 [batch] */
     uint64_t cu_q;          /* int32 [batch + 1], not decreasing */
     uint32_t batch;
-    uint32_t table_width;   /* valid entries of a table row: own tokens end at table_width * page_size */
+    uint32_t table_width;   /* valid entries of a table row: own tokens end at table_width * page_size, and at 2^31 - 256 */
     uint32_t table_stride;  /* entries from one row to the next */
     uint32_t tokens;        /* rows of the query, key, value and output operands */
 } tsw_kv_batch;

@@ -21,3 +21,12 @@ def probe(tmp_path_factory):
 def test_every_tile_once_and_every_part_found(probe, seed):
     r = subprocess.run([probe, str(seed + 11), "40"], capture_output=True, text=True, timeout=600)
     assert r.returncode == 0 and r.stdout.startswith("ok 40 cases"), (r.returncode, r.stdout[-500:], r.stderr[-1500:])
+
+
+def test_lengths_end_with_the_table_and_below_32_bits(tmp_path):
+    out = str(tmp_path / "kv_rows_probe")
+    r = subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-o", out,
+                        os.path.join(HERE, "kv_rows_probe.cpp")], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([out], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and r.stdout == "ok 10\n", (r.stdout, r.stderr)

@@ -146,7 +146,7 @@ int check_attention(const tsw_prefix_attention_args& a) {
     CHECK(check_batch(a.batch));
     CHECK(check_pages(a.cache, row, a.kv_heads, false, "cache"));
     if (a.prefix_len) {
-        if (a.prefix_len > 0x7fffff00u) return bad("prefix_len out of range");
+        if (a.prefix_len > (uint32_t)kMaxKeys) return bad("prefix_len out of range");
         if (!a.prefix_table || (a.prefix_table & 3)) return bad("prefix_table must be a 4-byte aligned device array");
         CHECK(check_pages(a.prefix, row, a.kv_heads, false, "prefix"));
     }

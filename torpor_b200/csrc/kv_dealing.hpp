@@ -30,8 +30,11 @@ constexpr int kTile = 128;                    // keys in a step, rows in a tile
 TSW_HD int imin(int a, int b) { return a < b ? a : b; }
 TSW_HD int imax(int a, int b) { return a > b ? a : b; }
 
+// Longest sequence: key numbers are 32 bits, and loops step past the end by less than 256.
+constexpr int kMaxKeys = 0x7fffff00;
+
 // Rows and length of one sequence, made safe: whatever the tables hold, 0 <= first, first + n <= tokens,
-// n <= max_q and 0 <= len <= what the page table covers.  Returns what had to be changed (TSW_KV_*).
+// n <= max_q and 0 <= len <= what the page table covers, kMaxKeys at most.  Returns what had to be changed (TSW_KV_*).
 struct SeqRows { int first, n, len; };
 TSW_HD uint32_t read_rows(const tsw_kv_batch& t, int b, uint32_t max_q, uint32_t page_size, SeqRows& r) {
     const int* cu = (const int*)t.cu_q;
@@ -45,7 +48,8 @@ TSW_HD uint32_t read_rows(const tsw_kv_batch& t, int b, uint32_t max_q, uint32_t
         r.first = 0;
         r.n = 0;
     }
-    const uint64_t room = t.page_table ? (uint64_t)t.table_width * page_size : 0;
+    uint64_t room = t.page_table ? (uint64_t)t.table_width * page_size : 0;
+    room = room < (uint64_t)kMaxKeys ? room : (uint64_t)kMaxKeys;
     if (len < 0) {
         bad |= TSW_KV_BAD_LENGTH;
         len = 0;
