@@ -434,3 +434,13 @@ def test_refusals_on_device_tensors():
     a = _cabi.KvAppendArgs()
     a.dtype = 9
     assert _cabi.lib().tsw_kv_append(0, a, None) == _cabi.ERR_INVALID
+
+
+def test_numbers_that_the_c_structures_would_cut_are_refused():
+    c = Batch([1], [4], prefix=16)
+    for offset in (-1, 1 << 32, (1 << 64) + 3):
+        with pytest.raises(ValueError, match="position_offset"):
+            kv_cache.kv_append(c.k_cache, c.v_cache, c.k, c.v, c.table, c.lens, c.cu_q, position_offset=offset)
+    for length in (-1, 0x7fffff01, (1 << 32) + 16):
+        with pytest.raises(ValueError, match="prefix_len"):
+            kv_cache.prefix_attention(c.q, c.k_cache, c.v_cache, c.table, c.lens, c.cu_q, prefix_table=c.prefix_table, prefix_len=length)

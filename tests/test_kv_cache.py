@@ -191,3 +191,22 @@ def test_frequencies():
     assert kv_cache.rope_frequencies(0, device="cpu").numel() == 0
     with pytest.raises(ValueError):
         kv_cache.rope_frequencies(7, device="cpu")
+
+
+def test_sizes_that_the_c_structures_would_cut_are_refused():
+    """Expanded tensors have such sizes without the memory."""
+    from torpor_b200 import kv_cache
+    cpu, half = torch.device("cpu"), torch.float16
+    x = torch.zeros(1, 1, 8, dtype=half)
+    for shape in ((2 ** 28 + 1, 1, 8), (2 ** 32 + 1, 1, 8), (1, 65537, 8), (1, 2 ** 32 + 1, 8)):
+        with pytest.raises(ValueError, match="at most"):
+            kv_cache._rows("q", x.expand(shape), half, cpu)
+    with pytest.raises(ValueError, match="at most"):
+        kv_cache._rows("q", torch.zeros(1, 1, 513, dtype=half), half, cpu)
+    for shape in ((2 ** 31, 1, 1, 8), (2 ** 32 + 1, 1, 1, 8), (1, 2 ** 20 + 1, 1, 8), (1, 2 ** 32 + 1, 1, 8), (1, 1, 4097, 8)):
+        with pytest.raises(ValueError, match="at most"):
+            kv_cache._pages(x[None].expand(shape), x[None].expand(shape), half, cpu, "cache")
+    i = torch.zeros(1, dtype=torch.int32)
+    many = torch.zeros(2 ** 24 + 1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="at most"):
+        kv_cache._batch(i[None].expand(2 ** 24, 1), many[:-1], many, 1, cpu)

@@ -34,6 +34,10 @@ def rope_frequencies(rotary_dim: int, theta: float = 10000.0, device="cuda") -> 
     return float(theta) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / max(rotary_dim, 1))
 
 
+# The C structures take 32 bits of a size without a word; what does not fit is refused here.
+_MAX_TOKENS = 1 << 28
+_MAX_KEYS = 0x7fffff00
+
 # The checks cost host time on calls that take a few microseconds on the device: messages are only put together
 # when they are raised.
 
@@ -50,6 +54,8 @@ def _rows(name: str, t: torch.Tensor, dtype, device):
     st = t.stride()
     if st[2] != 1 and shape[2] != 1:
         raise ValueError(f"{name}: the elements of a head must be contiguous")
+    if shape[0] > _MAX_TOKENS or shape[1] > 65536 or shape[2] > 512:
+        raise ValueError(f"{name}: at most 2^28 tokens, 65536 heads and 512 elements to a head")
     return t.data_ptr(), 2 * st[0], 2 * st[1], shape
 
 
@@ -60,6 +66,8 @@ def _pages(k: torch.Tensor, v: torch.Tensor, dtype, device, name: str) -> _cabi.
     ks, vs = k.stride(), v.stride()
     if (ks[3] != 1 or vs[3] != 1) and shape[3] != 1:
         raise ValueError(f"{name}: the elements of a head must be contiguous")
+    if shape[0] > 0x7fffffff or shape[1] > 1 << 20 or shape[2] > 4096:
+        raise ValueError(f"{name}: at most 2^31 - 1 pages of 2^20 tokens and 4096 heads")
     return _cabi.KvPages(k.data_ptr(), v.data_ptr(), 2 * ks[0], 2 * ks[1], 2 * ks[2], 2 * vs[0], 2 * vs[1], 2 * vs[2], shape[0], shape[1])
 
 
@@ -70,6 +78,8 @@ def _batch(page_table, seq_lens, cu_q, tokens: int, device) -> _cabi.KvBatch:
     n, (rows, width) = seq_lens.shape[0], page_table.shape
     if cu_q.shape[0] != n + 1 or rows != n:
         raise ValueError("page_table, seq_lens and cu_q disagree about the number of sequences")
+    if n > 0xffffff or width > 0xffffffff or page_table.stride(0) > 0xffffffff:
+        raise ValueError("at most 2^24 - 1 sequences, and 2^32 - 1 entries to a row of page_table")
     return _cabi.KvBatch(page_table.data_ptr(), seq_lens.data_ptr(), cu_q.data_ptr(), n, width, page_table.stride(0), tokens)
 
 
@@ -110,8 +120,8 @@ def kv_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: 
     tokens, heads, dim = shape
     if shape != v_shape or (heads, dim) != tuple(k_cache.shape[2:]):
         raise ValueError("k, v and the cache disagree about heads or head_dim")
-    if position_offset < 0:
-        raise ValueError("position_offset must not be negative")
+    if not 0 <= position_offset < 1 << 32:
+        raise ValueError("position_offset must be 0 to 2^32 - 1")
     a.batch = _batch(page_table, seq_lens, cu_q, tokens, device)
     if q is not None:
         a.q, a.q_token_stride, a.q_head_stride, q_shape = _rows("q", q, dtype, device)
@@ -163,8 +173,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if kv_shape[3] != dim:
         raise ValueError("q and the cache disagree about head_dim")
     a.batch = _batch(page_table, seq_lens, cu_q, tokens, device)
-    if prefix_len < 0:
-        raise ValueError("prefix_len must not be negative")
+    if not 0 <= prefix_len <= _MAX_KEYS:
+        raise ValueError("prefix_len must be 0 to 2^31 - 256")
     if prefix_len:
         if prefix_table is None:
             raise ValueError("a prefix needs its prefix_table")
