@@ -128,6 +128,23 @@ def test_operands_have_to_be_the_functions(function):
     torch.cuda.synchronize()
 
 
+def test_launches_are_counted(function):
+    eng, decode, model, block, _ = function
+    at = {t.name: model.tensor_vaddr[i] for i, t in enumerate(model.ws.tensors) if ".prompt." in t.name}
+    prompt = lambda l, what: at[f"model.layers.{l}.prompt.{what}"]
+    append, attention = decode._append(block, 0, 0), decode._attention(block, prompt, 0, 0)
+    rows = decode._attention(block, prompt, 0, 0)
+    rows.scale = 0.0                                # not for the tiles
+    for call, args, launches in ((eng.kv_append, append, 1), (eng.prefix_attention, attention, 2), (eng.prefix_attention, rows, 1)):
+        before = eng.stats()["kernel_launches"]
+        call("f", args)
+        assert eng.stats()["kernel_launches"] - before == launches
+        args.batch.tokens = 0
+        call("f", args)
+        assert eng.stats()["kernel_launches"] - before == launches
+    torch.cuda.synchronize()
+
+
 @pytest.mark.parametrize("call,side", [("kv_append", "cache"), ("prefix_attention", "cache"), ("prefix_attention", "prefix")])
 @pytest.mark.parametrize("field", ["k_page_stride", "v_page_stride"])
 def test_pages_that_pass_64_bits_leave_their_block(function, call, side, field):

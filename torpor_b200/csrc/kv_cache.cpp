@@ -93,6 +93,8 @@ int check_batch(const tsw_kv_batch& b) {
     return TSW_OK;
 }
 
+bool has_rows(const tsw_kv_batch& b) { return b.tokens && b.batch; }      // otherwise nothing is launched
+
 int check_heads(uint32_t dtype, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim) {
     if (dtype != TSW_F16 && dtype != TSW_BF16) return bad("dtype must be TSW_F16 or TSW_BF16");
     if (!kv_heads || kv_heads > 4096 || q_heads > 65536) return bad("head counts out of range");
@@ -241,7 +243,7 @@ int tsw_kv_append(int device, const tsw_kv_append_args* args, void* stream) {
         if (!args) return bad("null argument");
         if (device < 0 || device >= kMaxDevices) return bad("device ordinal out of range");
         CHECK(check_append(*args));
-        if (!args->batch.tokens || !args->batch.batch) return TSW_OK;
+        if (!has_rows(args->batch)) return TSW_OK;
         const DeviceGuard guard(device);
         int sms;
         CHECK(use_device(guard, device, &sms));
@@ -265,7 +267,7 @@ int tsw_prefix_attention(int device, const tsw_prefix_attention_args* args, void
         if (!args) return bad("null argument");
         if (device < 0 || device >= kMaxDevices) return bad("device ordinal out of range");
         CHECK(check_attention(*args));
-        if (!args->batch.tokens || !args->batch.batch) return TSW_OK;
+        if (!has_rows(args->batch)) return TSW_OK;
         const DeviceGuard guard(device);
         int sms;
         CHECK(use_device(guard, device, &sms));
@@ -324,7 +326,7 @@ int tsw_func_kv_append(tsw_engine* e, const char* func, const tsw_kv_append_args
         CHECK(operand(e, func, &a.v, span(row, a.batch.tokens, a.v_token_stride, a.kv_heads, a.v_head_stride), "v", stream));
         CHECK(operand(e, func, &a.inv_freq, 4ull * a.rotary_dim, "inv_freq", stream));
         const int rc = tsw_kv_append(e->cfg.device, &a, stream);
-        if (rc == TSW_OK) ++e->kernel_launches;
+        if (rc == TSW_OK && has_rows(a.batch)) ++e->kernel_launches;
         return rc;
     });
 }
@@ -350,7 +352,8 @@ int tsw_func_prefix_attention(tsw_engine* e, const char* func, const tsw_prefix_
         CHECK(operand(e, func, &a.lse, 4ull * a.batch.tokens * a.q_heads, "lse", stream));
         CHECK(operand(e, func, &a.workspace, a.workspace_bytes, "workspace", stream));
         const int rc = tsw_prefix_attention(e->cfg.device, &a, stream);
-        if (rc == TSW_OK) ++e->kernel_launches;
+        AttentionLayout w;
+        if (rc == TSW_OK && has_rows(a.batch)) e->kernel_launches += attention_layout(a, kMaxSms, &w) ? 2 : 1;      // tiles and joining, or rows
         return rc;
     });
 }
