@@ -63,3 +63,12 @@ def test_refusals(built):
     with pytest.raises(ValueError, match="GPU"):
         serving.SwapServer(1, 1 << 30, devices=[-1], decode_tokens=4)
     repo_reset()
+
+
+@pytest.mark.parametrize("wrong", [dict(decode_tokens=-1), dict(decode_tokens=4, prompt_tokens=0), dict(decode_tokens=4)])
+def test_a_server_that_refuses_has_made_no_engine(built, monkeypatch, wrong):
+    made = []
+    monkeypatch.setattr(serving, "MemoryManager", lambda *a, **kw: made.append(a))
+    with pytest.raises(ValueError):
+        serving.SwapServer(1, 1 << 30, devices=[-1], **wrong)
+    assert not made

@@ -140,6 +140,10 @@ class SwapServer:
                  shard_min_bytes: int = 0, decode_tokens: int = 0, prompt_tokens: int = 1024):
         self.n = n_gpus
         self.devices = devices or list(range(n_gpus))
+        if decode_tokens < 0 or prompt_tokens < 1:
+            raise ValueError("decode_tokens must not be negative, and a prompt has a token at least")
+        if decode_tokens and min(self.devices) < 0:
+            raise ValueError("decode_tokens needs engines on a GPU")
         self.engines = [MemoryManager(cap_bytes, device=self.devices[g], server_id=g, gpu_count=n_gpus,
                                       host_arena_bytes=host_arena_bytes if g == 0 else 0)
                         for g in range(n_gpus)]
@@ -161,8 +165,6 @@ class SwapServer:
         self.decode: Dict[str, tuple] = {}          # func -> (PromptDecode, its model, client address of its workspace block)
         self.streams = [0] * n_gpus
         if decode_tokens:
-            if min(self.devices) < 0:
-                raise ValueError("decode_tokens needs engines on a GPU")
             import torch
             self.streams = [torch.cuda.Stream(device=d) for d in self.devices]
 
