@@ -1,6 +1,9 @@
 """Key/value cache operators on a GPU: against 64-bit references, at the sizes and masks where they can go wrong."""
 import itertools
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -444,3 +447,32 @@ def test_numbers_that_the_c_structures_would_cut_are_refused():
     for length in (-1, 0x7fffff01, (1 << 32) + 16):
         with pytest.raises(ValueError, match="prefix_len"):
             kv_cache.prefix_attention(c.q, c.k_cache, c.v_cache, c.table, c.lens, c.cu_q, prefix_table=c.prefix_table, prefix_len=length)
+
+
+FIRST_CALL = """
+import sys
+sys.path[:0] = [{tests!r}, {root!r}]
+import torch
+from kv_cases import Batch
+from torpor_b200 import kv_cache
+c = Batch([1, 3], [40, 200], prefix=130, dim={dim}, seed=77)
+cache = c.k_cache.clone(), c.v_cache.clone()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    q = kv_cache.kv_append(*cache, c.k, c.v, c.table, c.lens, c.cu_q, q=c.q)
+    out = kv_cache.prefix_attention(q, c.k_cache, c.v_cache, c.table, c.lens, c.cu_q, max_q=3, prefix_table=c.prefix_table, prefix_len=130)
+graph.replay()
+torch.cuda.synchronize()
+c.check(out, q=q)
+assert kv_cache.kv_status(0) == 0
+print("captured")
+"""
+
+
+@pytest.mark.parametrize("dim", [64, 128, 200])
+def test_a_process_may_capture_its_first_call(dim):
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL.format(tests=here, root=os.path.dirname(here), dim=dim)], capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "captured", r.stderr[-2000:]
