@@ -94,8 +94,21 @@ __device__ __forceinline__ unsigned long long now() {
     return t;
 }
 // Every wait ends: after two seconds, or when another warp of the CTA has given up, it answers false, and the
-// caller leaves its loop.  The waiting itself is one copy: the kernel's code is fetched cold at every launch.
-__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {
+// caller leaves its loop.  Inlined: the call, though hardly ever made, costs the loops around it registers and
+// 2 % (4096 rows behind 16384 tokens).
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {           // a whole warp, one answer
+    if (__all_sync(~0u, mbar_try(bar, parity))) return true;
+    const unsigned long long t0 = now();
+    bool ok;
+#pragma unroll 1
+    do {
+        ok = mbar_try(bar, parity);
+        if (!ok && now() - t0 > kWaitNs) *gave_up = 1;
+    } while (!__all_sync(~0u, ok) && !__any_sync(~0u, *gave_up));
+    return __all_sync(~0u, ok);
+}
+__device__ __forceinline__ bool wait_alone(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {      // one thread
+    if (mbar_try(bar, parity)) return true;
     const unsigned long long t0 = now();
 #pragma unroll 1
     while (!mbar_try(bar, parity)) {
@@ -103,13 +116,6 @@ __device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile uin
         if (*gave_up) return false;
     }
     return true;
-}
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {           // a whole warp, one answer
-    if (__all_sync(~0u, mbar_try(bar, parity))) return true;
-    return __all_sync(~0u, wait_on(bar, parity, gave_up));
-}
-__device__ __forceinline__ bool wait_alone(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {      // one thread
-    return mbar_try(bar, parity) || wait_on(bar, parity, gave_up);
 }
 
 // One lane of a converged warp, chosen in a way that leaves the code under it uniform: operands of the tensor and
