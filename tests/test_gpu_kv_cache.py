@@ -169,6 +169,17 @@ def test_attention_long(dtype):
     c.check(out, lse)
 
 
+@pytest.mark.parametrize("q_heads,kv_heads,dim", [(6, 2, 64), (1, 1, 128)])
+def test_attention_many_tokens_without_a_prefix(q_heads, kv_heads, dim):
+    """Enough rows that the joining warps take a token each; rows that see nothing, rows of nobody, heads that are no
+    multiple of four, texts that end inside a row tile."""
+    c = Batch([3901, 0, 130, 70, 5], [3901, 9, 700, 33, 0], q_heads=q_heads, kv_heads=kv_heads, dim=dim, prefix=0, pad=3, first=2, seed=55)
+    out = torch.full_like(c.q, 7.0)
+    _, lse = attend(c, out=out, return_lse=True)
+    assert c.tokens >= 4096 and (out[:2] == 7).all() and (out[-3:] == 7).all()
+    c.check(out, lse)
+
+
 def test_attention_wide_batches_behind_a_prefix():
     c = Batch([1] * 200, [(i * 7) % 40 + 1 for i in range(200)], q_heads=8, kv_heads=2, dim=128, prefix=600, dtype=torch.bfloat16, seed=21)
     c.check(attend(c))
