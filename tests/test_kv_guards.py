@@ -1,0 +1,32 @@
+"""What the key/value cache kernels' shared code makes of unusual but legal calls and of wild tables, on the host: the probes
+include the very code that the kernels run."""
+import os
+import subprocess
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+def build(name, where):
+    out = str(where / name)
+    r = subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-o", out,
+                        os.path.join(HERE, name + ".cpp")], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    return out
+
+
+def run(*args):
+    r = subprocess.run([str(a) for a in args], capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0 and r.stdout.startswith("ok "), (r.returncode, r.stdout[-500:], r.stderr[-1500:])
+    return r.stdout
+
+
+@pytest.fixture(scope="module")
+def phases(tmp_path_factory):
+    return build("kv_phases_probe", tmp_path_factory.mktemp("phases"))
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_streams_know_every_phase_of_the_barriers_they_wait_for(phases, seed):
+    run(phases, seed + 1, 150)

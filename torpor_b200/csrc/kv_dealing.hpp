@@ -84,12 +84,15 @@ inline bool attention_layout(const tsw_prefix_attention_args& a, int sms, Attent
     w->ctas = sms;
     w->group = group;
     w->tile_tokens = std::min<uint32_t>(kTile / group, a.batch.tokens);
-    w->own_box_tokens = std::min(w->tile_tokens, std::max(1u, a.max_q));
+    // max_q is an upper bound and may pass the rows there are.  Cut to them, a list of own rows in pairs means a prefix list in
+    // pairs: a pair waits on the first stream's barriers for both, whose phases before it both have to know.
+    const uint32_t max_q = std::min(a.max_q, a.batch.tokens);
+    w->own_box_tokens = std::min(w->tile_tokens, std::max(1u, max_q));
     w->prefix_tiles = (a.prefix_len + kTile - 1) / kTile;
     // Two row tiles that share their key tiles, where there are two: with one, the streams of a CTA take
     // different key tiles.
     w->prefix_pair = a.batch.tokens > w->tile_tokens;
-    w->own_pair = a.max_q > w->tile_tokens;
+    w->own_pair = max_q > w->tile_tokens;
     w->part_rows = group * w->tile_tokens;
     // Tile numbers are 32 bits.
     const uint64_t row_tiles = (uint64_t)a.batch.tokens / w->tile_tokens + 1 + a.batch.batch;
