@@ -339,8 +339,9 @@ int tsw_place_segments_static_status(int device, void* stream, uint32_t* status,
  * on the host, leave the caller's current device as it was, and may be captured into a graph.  Bad
  * arguments that the host can see are refused with TSW_ERR_INVALID before anything is launched.  What
  * only the device sees -- a page number outside the cache, a length beyond the table, rows out of
- * order -- is never followed out of bounds: it is recorded in a word per device that
- * tsw_kv_status reads, and what was computed for that sequence is unspecified.  A page that
+ * order -- is never followed out of bounds: where a call comes across it, it is recorded in a word per device that
+ * tsw_kv_status reads, and what was computed for that sequence is unspecified (for a page of the prefix, or rows out of
+ * order: for any sequence).  A row is appended to a sequence whose rows contain it, or not at all.  A page that
  * takes new tokens belongs to one sequence: if two sequences name it, either's tokens may stay. */
 enum { TSW_F16 = 0, TSW_BF16 = 1 };
 typedef struct {

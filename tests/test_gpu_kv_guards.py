@@ -59,3 +59,40 @@ def test_max_q_may_be_any_upper_bound(q_lens, own, q_heads, kv_heads, dim, prefi
     for max_q in (c.tokens + 1, 16, 64, 200, 0x7fffffff):
         got = Call(c, max_q)()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), max_q
+
+
+BROKEN = [[0, 10, 12, 5], [0, 10, 12, 0], [0, 12, 10, 12], [9, 10, 12, 3]]
+
+
+@pytest.mark.parametrize("cu", BROKEN)
+def test_append_follows_no_row_into_a_sequence_that_does_not_have_it(cu):
+    """A row is appended to a sequence whose rows contain it, or not at all."""
+    c = Batch([10, 2, 0], [40, 30, 20], seed=3)
+    c.cu_q.copy_(torch.tensor(cu, dtype=torch.int32))
+    want_k, want_v = c.k_cache.clone(), c.v_cache.clone()
+    other_k, other_v = want_k.clone(), want_v.clone()
+    for tok in range(c.tokens):
+        for b in range(3):
+            if not cu[b] <= tok < cu[b + 1]:
+                continue
+            j = c.own[b] - (cu[b + 1] - cu[b]) + tok - cu[b]
+            want_k[int(c.table[b, j // 16]), j % 16], want_v[int(c.table[b, j // 16]), j % 16] = c.k[tok], c.v[tok]
+            break
+    kv_cache.kv_append(c.k_cache, c.v_cache, c.k, c.v, c.table, c.lens, c.cu_q)
+    assert kv_cache.kv_status(0, clear=True) in (0, kv_cache.BAD_ROWS)
+    # a row that two overlapping sequences claim may be found in either
+    changed = (c.k_cache != other_k).flatten(2).any(-1)
+    assert (changed <= (want_k != other_k).flatten(2).any(-1)).all()
+    if cu == BROKEN[0]:
+        assert torch.equal(c.k_cache, want_k) and torch.equal(c.v_cache, want_v)
+
+
+@pytest.mark.parametrize("cu", BROKEN)
+@pytest.mark.parametrize("prefix,dim,causal", [(0, 64, True), (300, 128, True), (300, 64, False), (20, 200, True)])
+def test_attention_with_rows_out_of_order_is_recorded_and_stays_in_bounds(cu, prefix, dim, causal):
+    c = Batch([10, 2, 0], [400, 300, 200], dim=dim, prefix=prefix, seed=4, pad=2)
+    c.cu_q.copy_(torch.tensor(cu, dtype=torch.int32))
+    kv_cache.prefix_attention(c.q, c.k_cache, c.v_cache, c.table, c.lens, c.cu_q, max_q=12, causal=causal, prefix_len=prefix,
+                              prefix_table=c.prefix_table if prefix else None)
+    # the tile kernel looks at every sequence, the row kernel (wide heads) at those that it finds rows in
+    assert kv_cache.kv_status(0, clear=True) in ((0, kv_cache.BAD_ROWS) if dim > 128 else (kv_cache.BAD_ROWS,))

@@ -30,3 +30,13 @@ def phases(tmp_path_factory):
 @pytest.mark.parametrize("seed", range(4))
 def test_streams_know_every_phase_of_the_barriers_they_wait_for(phases, seed):
     run(phases, seed + 1, 150)
+
+
+@pytest.fixture(scope="module")
+def search(tmp_path_factory):
+    return build("kv_search_probe", tmp_path_factory.mktemp("search"))
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_a_row_is_only_looked_for_where_its_sequence_has_it(search, seed):
+    run(search, seed + 1, 300)

@@ -30,6 +30,14 @@ constexpr int kTile = 128;                    // keys in a step, rows in a tile
 TSW_HD int imin(int a, int b) { return a < b ? a : b; }
 TSW_HD int imax(int a, int b) { return a > b ? a : b; }
 
+TSW_HD uint32_t trailing_ones(uint32_t x) {
+#ifdef __CUDA_ARCH__
+    return __clz(__brev(~x));
+#else
+    return ~x ? __builtin_ctz(~x) : 32;
+#endif
+}
+
 // Longest sequence: key numbers are 32 bits, and loops step past the end by less than 256.
 constexpr int kMaxKeys = 0x7fffff00;
 
@@ -61,6 +69,26 @@ TSW_HD uint32_t read_rows(const tsw_kv_batch& t, int b, uint32_t max_q, uint32_t
     r.len = len;
     return bad;
 }
+
+// The sequence whose rows contain a token, looked for by 32 lanes that narrow the range 32-fold a step.  Whatever the table holds,
+// cu_q[lo - 1] <= tok and cu_q[hi] > tok (where there are such entries) hold from step to step, so a sequence that is
+// found has cu_q[b] <= tok < cu_q[b + 1]: only the lanes in front of the first one that sees a later row move lo.
+struct Search {
+    uint32_t lo, hi;
+    TSW_HD explicit Search(uint32_t batch) : lo(0), hi(batch + 1) {}
+    TSW_HD bool open() const { return lo < hi; }
+    TSW_HD uint32_t step() const { return (hi - lo + 31) / 32; }
+    TSW_HD bool vote(const int* cu_q, int tok, int lane) const {      // the first entry of this lane's piece
+        const uint32_t at = lo + lane * step();
+        return at < hi && cu_q[at] <= tok;
+    }
+    TSW_HD void take(uint32_t votes) {
+        const uint32_t by = step(), lead = trailing_ones(votes);
+        hi = (uint32_t)imin((int)hi, (int)(lo + lead * by));
+        if (lead) lo += (lead - 1) * by + 1;
+    }
+    TSW_HD int sequence(uint32_t batch) const { return lo <= batch ? (int)lo - 1 : -1; }
+};
 
 // ------------------------------------------------------------------ which calls, and their layout
 

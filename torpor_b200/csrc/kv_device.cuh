@@ -30,26 +30,12 @@ __device__ __forceinline__ float warp_sum(float x) {
     return x;
 }
 
-// The sequence whose rows contain `tok`, or -1: the last b with cu_q[b] <= tok, if tok < cu_q[b + 1].
-// All lanes of a warp call it; each step narrows the range 32-fold.
+// The sequence whose rows contain `tok`, or -1 (kv_dealing.hpp).  All lanes of a warp call it.
 __device__ __forceinline__ int find_sequence(const int* cu_q, uint32_t batch, uint32_t tok) {
-    const int lane = threadIdx.x & 31;
-    uint32_t lo = 0, hi = batch + 1;              // entries [0, lo) are <= tok (lo >= 1 once any is), [hi, ..) are > tok
+    Search s(batch);
 #pragma unroll 1
-    while (lo < hi) {
-        const uint32_t span = hi - lo, step = (span + 31) / 32;
-        const uint32_t at = lo + lane * step;     // first entry of this lane's piece
-        const bool below = at < hi && cu_q[at] <= (int)tok;
-        const unsigned votes = __ballot_sync(~0u, below);
-        const int k = __popc(votes);              // pieces whose first entry is <= tok: a prefix when cu_q does not decrease
-        if (k == 0) break;
-        const uint32_t next_lo = lo + (k - 1) * step + 1;
-        hi = min(hi, lo + k * step);
-        lo = next_lo;
-    }
-    const int b = (int)lo - 1;
-    if (b < 0 || b >= (int)batch) return -1;
-    return b;
+    while (s.open()) s.take(__ballot_sync(~0u, s.vote(cu_q, (int)tok, threadIdx.x & 31)));
+    return s.sequence(batch);
 }
 
 }  // namespace tsw
