@@ -96,3 +96,16 @@ def test_attention_with_rows_out_of_order_is_recorded_and_stays_in_bounds(cu, pr
                               prefix_table=c.prefix_table if prefix else None)
     # the tile kernel looks at every sequence, the row kernel (wide heads) at those that it finds rows in
     assert kv_cache.kv_status(0, clear=True) in ((0, kv_cache.BAD_ROWS) if dim > 128 else (kv_cache.BAD_ROWS,))
+
+
+def test_rows_claimed_by_very_many_sequences_are_recorded_and_not_dealt_out():
+    """131072 sequences that all name the same 8192 rows: more tiles than 32 bits count."""
+    tokens, heads, batch, keys = 8192, 32, 131072, 32768
+    q = torch.randn(tokens, heads, 8, device="cuda").half()
+    k, v = torch.randn(2, 4, 128, heads, 8, device="cuda").half()
+    cu = torch.zeros(batch + 1, dtype=torch.int32, device="cuda")
+    cu[1::2] = tokens
+    table = torch.zeros(batch, keys // 128, dtype=torch.int32, device="cuda")
+    lens = torch.full((batch,), keys, dtype=torch.int32, device="cuda")
+    kv_cache.prefix_attention(q, k, v, table, lens, cu, max_q=tokens, causal=False)
+    assert kv_cache.kv_status(0, clear=True) == kv_cache.BAD_ROWS

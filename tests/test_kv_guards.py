@@ -40,3 +40,7 @@ def search(tmp_path_factory):
 @pytest.mark.parametrize("seed", range(4))
 def test_a_row_is_only_looked_for_where_its_sequence_has_it(search, seed):
     run(search, seed + 1, 300)
+
+
+def test_tile_numbers_stay_within_32_bits(tmp_path):
+    run(build("kv_totals_probe", tmp_path))

@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
     for (uint32_t b = b_lo; b < b_hi; ++b) {
         SeqRows r;
         wrong |= read_rows(a.batch, b, a.max_q, a.cache.page_size, r);
-        mine += sequence_tiles(d, r);
+        mine = add_tiles(mine, sequence_tiles(d, r));
     }
     if (warp == kWarpSchedule) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const uint32_t up = __shfl_up_sync(~0u, before, o);
-        if (lane >= o) before += up;
+        if (lane >= o) before = add_tiles(before, up);
     }
     if (lane == 31) s_scan[warp] = before;
     before -= mine;
@@ -303,8 +303,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
 #pragma unroll
     for (int i = 0; i < (kThreads + 31) / 32; ++i) {
         if (i == warp) before += total;
-        total += s_scan[i];
+        total = add_tiles(total, s_scan[i]);
     }
+    if (countable(total) != total && blockIdx.x == 0 && tid == 0) atomicOr(p.status, TSW_KV_BAD_ROWS);
+    total = countable(total);
     if (warp == kWarpSchedule) {
         int tok0, tok1;
         const uint32_t rts = prefix_rows(d, tok0, tok1), prefix_total = a.kv_heads * rts * w.prefix_tiles;

@@ -38,6 +38,12 @@ TSW_HD uint32_t trailing_ones(uint32_t x) {
 #endif
 }
 
+// Tiles of a list.  Sequences that keep apart stay below this (attention_layout sees to it); rows claimed by many sequences of
+// a wild table may not: their sum stops here, and a list that got so far is not dealt out at all.
+constexpr uint32_t kMaxTiles = 0x7fffffff;
+TSW_HD uint32_t add_tiles(uint32_t a, uint32_t b) { return a + b < kMaxTiles ? a + b : kMaxTiles; }      // a, b <= kMaxTiles
+TSW_HD uint32_t countable(uint32_t total) { return total < kMaxTiles ? total : 0; }
+
 // Longest sequence: key numbers are 32 bits, and loops step past the end by less than 256.
 constexpr int kMaxKeys = 0x7fffff00;
 
@@ -122,10 +128,11 @@ inline bool attention_layout(const tsw_prefix_attention_args& a, int sms, Attent
     w->prefix_pair = a.batch.tokens > w->tile_tokens;
     w->own_pair = max_q > w->tile_tokens;
     w->part_rows = group * w->tile_tokens;
-    // Tile numbers are 32 bits.
+    // Tile numbers are 32 bits; no sequence is longer than kMaxKeys, however wide its table.
     const uint64_t row_tiles = (uint64_t)a.batch.tokens / w->tile_tokens + 1 + a.batch.batch;
-    const uint64_t own_tiles = ((uint64_t)a.batch.table_width * a.cache.page_size + kTile - 1) / kTile;
-    if (a.kv_heads * row_tiles * std::max<uint64_t>(own_tiles, w->prefix_tiles) >> 31) return false;
+    const uint64_t own_keys = std::min<uint64_t>((uint64_t)a.batch.table_width * a.cache.page_size, kMaxKeys);
+    const uint64_t tiles = std::max<uint64_t>((own_keys + kTile - 1) / kTile, w->prefix_tiles);
+    if (tiles && a.kv_heads * row_tiles > kMaxTiles / tiles) return false;
     uint64_t at = 0;
     auto part = [&](uint64_t bytes) {
         const uint64_t here = at;
@@ -451,7 +458,7 @@ TSW_HD Parts own_parts(const Deal& d, const SeqRows& r, int tok, int kv_head, ui
     Parts p = {};
     const Cut c = cut_own(d, r, split_rows(d, d.w.own_pair, tok - r.first, p));
     const int seen = p.half ? c.kt_b : c.kt_a;
-    if (!seen) return p;
+    if (!seen || !total) return p;
     const uint32_t x = base + before * d.kv_heads + kv_head * imax(c.kt_a, c.kt_b), n = ranges(d, d.w.own_pair, total);
     p.has = true;
     p.first = range_of(x, total, n);
