@@ -109,3 +109,25 @@ def test_rows_claimed_by_very_many_sequences_are_recorded_and_not_dealt_out():
     lens = torch.full((batch,), keys, dtype=torch.int32, device="cuda")
     kv_cache.prefix_attention(q, k, v, table, lens, cu, max_q=tokens, causal=False)
     assert kv_cache.kv_status(0, clear=True) == kv_cache.BAD_ROWS
+
+
+@pytest.mark.parametrize("q_lens,max_q,pad", [([5], 3, 0), ([200], 100, 40)])
+def test_what_follows_on_the_stream_comes_after_both_kernels(q_lens, max_q, pad):
+    """No row has anything to join (its sequence has more rows than max_q), while the tile kernel walks a long prefix for them: its
+    workspace and its report are complete for whatever the stream does next."""
+    c = Batch(q_lens, [400], q_heads=32, kv_heads=32, dim=128, prefix=40000, page_size=64, pad=pad, seed=6)
+    c.prefix_table[-1] = c.pages                       # seen last, in the range that ends the list
+    call = Call(c, max_q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            call.workspace.fill_(0xFF)
+            call()
+            behind = call.workspace.clone()
+            word = kv_cache.kv_status(0, side.cuda_stream, clear=True)
+        torch.cuda.synchronize()
+        assert word == kv_cache.BAD_ROWS | kv_cache.BAD_PAGE
+        assert kv_cache.kv_status(0) == 0
+        assert torch.equal(behind, call.workspace)
+        assert (call.out == 5.0).all()

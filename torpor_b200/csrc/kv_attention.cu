@@ -739,13 +739,15 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(const __grid_cons
     constexpr int kVec = DP / 32;                    // float4s of a lane: element 4 * (sub + 8 * i)
     const int lane = threadIdx.x & 31, sub = lane & 7, warp = threadIdx.x >> 5;
     const int tok = many ? (int)(blockIdx.x * kJoinWarps) + warp : (int)blockIdx.x;
-    if (tok >= (int)a.batch.tokens) return;
     const AttentionLayout& w = d.w;
-    const int b = find_sequence((const int*)a.batch.cu_q, a.batch.batch, tok);
-    if (b < 0) return;
-    SeqRows r;
-    read_rows(a.batch, b, a.max_q, a.cache.page_size, r);
-    if (tok >= r.first + r.n) return;
+    const int b = tok < (int)a.batch.tokens ? find_sequence((const int*)a.batch.cu_q, a.batch.batch, tok) : -1;
+    SeqRows r = {};
+    if (b >= 0) read_rows(a.batch, b, a.max_q, a.cache.page_size, r);
+    if (b < 0 || tok >= r.first + r.n) {
+        // Nothing to join, but what comes behind on the stream is ordered behind this grid alone: it ends after the tile kernel.
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     uint32_t before = 0;
 #pragma unroll 1
     for (int rt = (int)((uint32_t)(tok - r.first) / (uint32_t)own_item_tokens(d)), i = lane; i < rt; i += 32) {
