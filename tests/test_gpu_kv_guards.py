@@ -131,3 +131,32 @@ def test_what_follows_on_the_stream_comes_after_both_kernels(q_lens, max_q, pad)
         assert kv_cache.kv_status(0) == 0
         assert torch.equal(behind, call.workspace)
         assert (call.out == 5.0).all()
+
+
+def long_list(n, page_size):
+    """``n`` keys that name two pages over and over, values 0 in the first half of the list and 1 in the second: (table, keys, values)."""
+    pages_ = -(-n // page_size)
+    table = torch.zeros(pages_, dtype=torch.int32, device="cuda")
+    table[pages_ // 2:] = 1
+    k = torch.zeros(2, page_size, 1, 8, dtype=torch.float16, device="cuda")
+    v = torch.stack((torch.zeros_like(k[0]), torch.ones_like(k[0])))
+    return table, k, v
+
+
+@pytest.mark.parametrize("where", ["prefix", "own"])
+@pytest.mark.parametrize("n", [0x7fffff00, (1 << 30) + (1 << 29) + 77])
+def test_lists_longer_than_two_to_the_thirtieth(where, n):
+    """Equal scores, so the result is the share of the second half and the log-sum is ln n.  Sums of equal powers of two are exact in
+    32 bits up to 2^24 of them; joining up to 300 of them rounds each time by 2^-24 at most, the result once."""
+    ps = 1 << 20
+    table, k, v = long_list(n, ps)
+    q = torch.randn(3, 1, 8, device="cuda").half()
+    cu = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    if where == "prefix":
+        out, lse = kv_cache.prefix_attention(q, k, v, torch.zeros(1, 0, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"),
+                                             cu, prefix_table=table, prefix_len=n, return_lse=True)
+    else:
+        out, lse = kv_cache.prefix_attention(q, k, v, table[None], torch.tensor([n], dtype=torch.int32, device="cuda"), cu, causal=False, return_lse=True)
+    want = (n - len(table) // 2 * ps) / n
+    assert (out.double() - want).abs().max() <= want * (2.0 ** -11 + 300 * 2.0 ** -23)
+    assert (lse.double() - torch.tensor(float(n)).double().log().cuda()).abs().max() <= 300 * 2.0 ** -24 + 2.0 ** -22 * 23

@@ -44,3 +44,7 @@ def test_a_row_is_only_looked_for_where_its_sequence_has_it(search, seed):
 
 def test_tile_numbers_stay_within_32_bits(tmp_path):
     run(build("kv_totals_probe", tmp_path))
+
+
+def test_a_row_sees_all_keys_its_mask_leaves_it(tmp_path):
+    run(build("kv_seen_probe", tmp_path))

@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
             const int tok = j.tok + tok_in_tile;
             const bool mine = tok_in_tile < j.tokens;
             const bool warp_on = (warp & 3) * 32 < j.tokens * group;
-            int left = min(j.keys, max(0, j.limit + tok));                // keys this row sees from here on
+            int left = keys_seen(j, tok);                                 // keys this row sees from here on
             float top = -INFINITY, sum = 0.f;
 #pragma unroll 1
             for (int unit = 0; unit < j.units; ++unit, ++count, left -= kHalf) {

@@ -210,9 +210,9 @@ struct Job {
     int kt0, kt1;            // key tiles of this range
     int kt_a, kt_b;          // ends of what the two row tiles see
     int keys;                // keys of the whole segment
-    int limit;               // row of token t sees keys below limit + t + 1
+    int limit;               // row of token t sees keys below limit + t + 1; kNoLimit: all of them
 };
-constexpr int kNoLimit = 0x3fffffff;
+constexpr int kNoLimit = 0x7fffffff;          // above every other limit: lengths end at kMaxKeys
 
 struct Start { int b, rt, head, kt; uint32_t left; };      // where a stream's own range begins, and its tiles
 
@@ -412,7 +412,7 @@ TSW_HD uint32_t make_take(const Job& j, int tile, bool use, bool pair, uint32_t 
 // A stream's share of a job: its rows, how many units, and where the result goes.
 struct alignas(16) RowJob {
     int head, tok, tokens, units;    // units = 0: no more
-    int keys, limit;                 // from the range's first key: row of token t sees keys below min(keys, limit + t)
+    int keys, limit;                 // from the range's first key: row of token t sees keys below min(keys, limit + t), or all (kNoLimit)
     int own, place;                  // place >= 0: partial result of a range that continues an item
 };
 enum { kPlaceDirect = -2, kPlaceHome = -1 };
@@ -427,11 +427,14 @@ TSW_HD RowJob make_row_job(const Deal& d, const Job& j, bool pair, int s, uint32
     r.tokens = pair && s ? j.n_b : j.n_a;
     r.units = 2 * (end - j.kt0 - 1) + units_of(tile_keys(j, end - 1));
     r.keys = j.keys - j.kt0 * kTile;
-    r.limit = j.limit + 1 - j.kt0 * kTile;
+    r.limit = j.limit == kNoLimit ? kNoLimit : j.limit + 1 - j.kt0 * kTile;
     r.own = j.own;
     r.place = j.kt0 ? (int)part_place(pair, range_index(d, pair, cta, s), s) : !d.prefix_len && end == seen ? (int)kPlaceDirect : (int)kPlaceHome;
     return r;
 }
+
+// Keys from the range's first one on that the row of token `tok` sees.
+TSW_HD int keys_seen(const RowJob& j, int tok) { return j.limit == kNoLimit ? j.keys : imin(j.keys, imax(0, j.limit + tok)); }
 
 // Where the partial results of one row lie: of each list the ranges first .. last, its half of a pair and its
 // token's place in the row tile.  `before`: own tiles of the row's sequence in front of its item (one head).
