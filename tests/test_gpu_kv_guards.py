@@ -1,5 +1,6 @@
 """Key/value cache operators on a GPU: legal calls at the edges of what the arguments allow."""
 import ctypes as C
+import math
 
 import pytest
 import torch
@@ -160,3 +161,38 @@ def test_lists_longer_than_two_to_the_thirtieth(where, n):
     want = (n - len(table) // 2 * ps) / n
     assert (out.double() - want).abs().max() <= want * (2.0 ** -11 + 300 * 2.0 ** -23)
     assert (lse.double() - torch.tensor(float(n)).double().log().cuda()).abs().max() <= 300 * 2.0 ** -24 + 2.0 ** -22 * 23
+
+
+def one_key_and_a_tail(n, share, dtype, where, heads=1, dim=64):
+    """Key 7 takes ``share`` of the weight, the others an equal part of the rest each; its value is 0, theirs 1.
+    Returns the call's results and what they are in 64 bits."""
+    u = 8.0
+    score = math.log(share / (1 - share) * (n - 1))
+    q = torch.zeros(1, heads, dim, device="cuda", dtype=dtype)
+    q[..., 0] = u
+    pages_ = -(-n // 256)
+    k = torch.zeros(pages_ + 1, 256, heads, dim, device="cuda", dtype=dtype)
+    v = torch.ones_like(k)
+    k[0, 7, :, 0], v[0, 7] = score / u, 0.0
+    score = u * k[0, 7, 0, 0].double().item()
+    table, cu = torch.arange(pages_, dtype=torch.int32, device="cuda"), torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([n if where == "own" else 0], dtype=torch.int32, device="cuda")
+    out, lse = kv_cache.prefix_attention(q, k, v, table[None], lens, cu, max_q=1, scale=1.0, return_lse=True,
+                                         **(dict(prefix_table=table, prefix_len=n) if where == "prefix" else {}))
+    w = math.exp(score)
+    return out, lse, (n - 1) / (w + n - 1), math.log(w + n - 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("where", ["prefix", "own"])
+@pytest.mark.parametrize("n", [1 << 15, 1 << 18, 1 << 20, (1 << 22) + 5])
+@pytest.mark.parametrize("share", [0.9, 0.99])
+def test_a_flat_tail_behind_one_key_counts(dtype, where, n, share):
+    """Weights far below the largest add up.  Each is rounded once (to 16 bits, half a step relative; in fp16 to 2^-36 of the largest
+    at worst, where its steps are equal), the result once more; the exponential and its argument (up to 21, in 32 bits)
+    take 2^-18, the sums of n / 64 / 148 units and 148 ranges 2^-13 at most."""
+    out, lse, want, want_lse = one_key_and_a_tail(n, share, dtype, where)
+    u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
+    tol = want * (2.01 * u + 2.0 ** -18 + 2.0 ** -13) + (n * share * 2.0 ** -36 if dtype is torch.float16 else 0.0)
+    assert (out.double() - want).abs().max().item() <= tol, (out.double().flatten()[0].item(), want)
+    assert abs(lse.item() - want_lse) <= 2.0 ** -13 + 2.0 ** -18

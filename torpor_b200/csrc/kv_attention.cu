@@ -4,7 +4,7 @@
 // 128.  S = Q K^T and O += P V are tcgen05.mma chains (M = 128; accumulators in tensor memory, the weights P go back
 // into tensor memory over S and are the A operand of the second product).  One thread holds one row of S: maximum,
 // exponentials and sum need no exchange between threads.  The maximum that exponentials are taken against
-// moves only when it grows by more than 2^8, so the running output is rarely rescaled; the quotient at the
+// moves only when it grows by more than 2^8 (fp16: 2^4), so the running output is rarely rescaled; the quotient at the
 // end makes the result independent of it.  Weights are rounded to the operands' 16 bits, which the
 // tensor cores take; their sum is formed from the unrounded 32-bit values, as are maximum and output.
 //
@@ -46,7 +46,13 @@ namespace {
 
 constexpr int kThreads = 416;                 // two warpgroups of rows; warps for keys, values, each stream's products, scheduling
 constexpr unsigned long long kWaitNs = 2000000000ull, kDrainNs = 5000000ull;
-constexpr float kGrow = 8.f;                  // log2 of the growth of the maximum that is let pass
+// log2 of the growth of the maximum that is let pass, and of the weight that the maximum's own key has.  bf16 reaches as far down as
+// 32 bits do.  fp16 ends at 2^-24, and a weight of 1 for the maximum would leave what lies above unused: a flat tail of a
+// million keys behind one that takes 90 % lost an eighth.  Raised by 2^11 (with the growth 2^15, the type ends at 2^16) a weight loses
+// bits from 2^-25 of the maximum's on and is lost at 2^-36, where 32-bit sums over as many keys no longer show it.
+// A growth of 2^4 instead of 2^8 is exceeded, behind random keys, in 1 of 20 warps and items.
+template <typename T> constexpr float kGrow = std::is_same<T, __half>::value ? 4.f : 8.f;
+template <typename T> constexpr float kRaise = std::is_same<T, __half>::value ? 11.f : 0.f;
 
 template <int DP> struct Shape {
     static constexpr int kTileBytes = kTile * DP * 2;
@@ -604,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
                     if (unit == 0) {
                         top = here;
                     } else {
-                        const bool grow = (here - top) * c > kGrow;              // also from -inf; never between two of them
+                        const bool grow = (here - top) * c > kGrow<T>;              // also from -inf; never between two of them
                         if (__any_sync(~0u, grow)) {
                             const float f = grow ? exp2_fast((top - here) * c) : 1.f;
                             if (grow) top = here;
@@ -623,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
                             }
                         }
                     }
-                    const float base = top == -INFINITY ? 0.f : top * c;
+                    const float base = top == -INFINITY ? 0.f : top * c - kRaise<T>;
                     const uint64_t c2 = two(c, c), base2 = two(-base, -base);
                     uint64_t s0 = 0, s1 = 0;
 #pragma unroll
@@ -680,12 +686,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
                 if (j.place == kPlaceDirect) {
                     out = (uint8_t*)(a.out + (uint64_t)tok * a.out_token_stride + (uint64_t)head * a.out_head_stride);
                     f = sum == 0.f ? 0.f : 1.f / sum;
-                    if (a.lse) ((float*)a.lse)[row_at] = sum == 0.f ? -INFINITY : (top * c + log2f(sum)) * 0.6931471805599453f;
+                    if (a.lse) ((float*)a.lse)[row_at] = sum == 0.f ? -INFINITY : (top * c - kRaise<T> + log2f(sum)) * 0.6931471805599453f;
                 } else {
                     const bool home = j.place == kPlaceHome;
                     const uint64_t at = home ? home_index(d, j.own, row_at, a.q_heads) : part_index(d, j.own, j.place, row);
                     out = ws + (home ? w.home_o : w.part_o) + 4 * at * a.head_dim;
-                    *((float2*)(ws + (home ? w.home_ml : w.part_ml)) + at) = make_float2(top == -INFINITY ? -INFINITY : top * c, sum);
+                    *((float2*)(ws + (home ? w.home_ml : w.part_ml)) + at) = make_float2(top == -INFINITY ? -INFINITY : top * c - kRaise<T>, sum);
                 }
             }
 #pragma unroll 1
