@@ -67,6 +67,7 @@ int main() {
         }
         const uint32_t total = countable(sum);
         REQUIRE(total == (all < kMaxTiles ? all : 0));
+        if (!total) std::fill(base.begin(), base.end(), 0);
         // no range goes past the last sequence, and no row's parts past the workspace
         for (uint32_t cta = 0; cta < w.ctas; ++cta)
             for (int s = 0; s < 2; ++s) {
@@ -84,9 +85,8 @@ int main() {
                         const Cut c = cut_own(d, r, i);
                         before += std::max(c.kt_a, c.kt_b);
                     }
-                    const Parts p = own_parts(d, r, tok, kv, base[b], before, total);
-                    REQUIRE(p.has == (total != 0));
-                    if (p.has) REQUIRE(p.first <= p.last && part_place(w.own_pair, p.last, p.half) < 2 * w.ctas);
+                    const Parts p = own_parts(d, r, tok, kv, base[b], before, sum);
+                    REQUIRE(p.has && p.first <= p.last && part_place(w.own_pair, p.last, p.half) < 2 * w.ctas);
                     ++checks;
                 }
     }

@@ -311,8 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
         if (i == warp) before += total;
         total = add_tiles(total, s_scan[i]);
     }
-    if (countable(total) != total && blockIdx.x == 0 && tid == 0) atomicOr(p.status, TSW_KV_BAD_ROWS);
-    total = countable(total);
+    const bool too_many = countable(total) != total;
     if (warp == kWarpSchedule) {
         int tok0, tok1;
         const uint32_t rts = prefix_rows(d, tok0, tok1), prefix_total = a.kv_heads * rts * w.prefix_tiles;
@@ -324,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
             if (blockIdx.x == 0) {                    // for the joining kernel
                 uint32_t* base = (uint32_t*)((uint8_t*)a.workspace + w.own_base);
                 base[batch] = total;
+                if (too_many) atomicOr(p.status, TSW_KV_BAD_ROWS);
                 base[batch + 1] = prefix_total;
             }
         }
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
         uint32_t at = before;
 #pragma unroll 1
         for (uint32_t b = b_lo; b < b_hi; ++b) {
-            base[b] = at;
+            base[b] = too_many ? 0 : at;
             SeqRows r;
             read_rows(a.batch, b, a.max_q, a.cache.page_size, r);
             at += sequence_tiles(d, r);
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
     }
 #pragma unroll 1
     for (int s = 0; s < 2; ++s) {
-        const Range g = range_at(d, w.own_pair, total, blockIdx.x, s);
+        const Range g = range_at(d, w.own_pair, countable(total), blockIdx.x, s);
         if (g.end > g.x && g.x >= before && g.x < before + mine) find_start(d, b_lo, b_hi, g.x - before, g.end - g.x, s_pro.own[s]);
     }
     fence_before();

@@ -39,7 +39,8 @@ TSW_HD uint32_t trailing_ones(uint32_t x) {
 }
 
 // Tiles of a list.  Sequences that keep apart stay below this (attention_layout sees to it); rows claimed by many sequences of
-// a wild table may not: their sum stops here, and a list that got so far is not dealt out at all.
+// a wild table may not: their sum stops here, and a list that got so far is not dealt out at all.  For the joining kernel
+// every sequence then begins at 0 of kMaxTiles, which keeps what it works out inside its tables without a look of its own.
 constexpr uint32_t kMaxTiles = 0x7fffffff;
 TSW_HD uint32_t add_tiles(uint32_t a, uint32_t b) { return a + b < kMaxTiles ? a + b : kMaxTiles; }      // a, b <= kMaxTiles
 TSW_HD uint32_t countable(uint32_t total) { return total < kMaxTiles ? total : 0; }
@@ -461,7 +462,7 @@ TSW_HD Parts own_parts(const Deal& d, const SeqRows& r, int tok, int kv_head, ui
     Parts p = {};
     const Cut c = cut_own(d, r, split_rows(d, d.w.own_pair, tok - r.first, p));
     const int seen = p.half ? c.kt_b : c.kt_a;
-    if (!seen || !total) return p;
+    if (!seen) return p;
     const uint32_t x = base + before * d.kv_heads + kv_head * imax(c.kt_a, c.kt_b), n = ranges(d, d.w.own_pair, total);
     p.has = true;
     p.first = range_of(x, total, n);
