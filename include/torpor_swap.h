@@ -341,7 +341,7 @@ int tsw_place_segments_static_status(int device, void* stream, uint32_t* status,
  * only the device sees -- a page number outside the cache, a length beyond the table, rows out of
  * order -- is never followed out of bounds: where a call comes across it, it is recorded in a word per device that
  * tsw_kv_status reads, and what was computed for that sequence is unspecified (for a page of the prefix, or rows out of
- * order: for any sequence).  A row is appended to a sequence whose rows contain it, or not at all.  A page that
+ * order: for any sequence).  A row is appended to a sequence whose rows contain it and whose length the table covers, or not at all.  A page that
  * takes new tokens belongs to one sequence: if two sequences name it, either's tokens may stay. */
 enum { TSW_F16 = 0, TSW_BF16 = 1 };
 typedef struct {

@@ -196,3 +196,19 @@ def test_a_flat_tail_behind_one_key_counts(dtype, where, n, share):
     tol = want * (2.01 * u + 2.0 ** -18 + 2.0 ** -13) + (n * share * 2.0 ** -36 if dtype is torch.float16 else 0.0)
     assert (out.double() - want).abs().max().item() <= tol, (out.double().flatten()[0].item(), want)
     assert abs(lse.item() - want_lse) <= 2.0 ** -13 + 2.0 ** -18
+
+
+@pytest.mark.parametrize("lens", [[65, 33], [66, 33], [2**31 - 1, 33], [-1, 33]])
+def test_append_beyond_the_table_overwrites_nothing(lens):
+    """A sequence that has outgrown its table: the new token has no place, and the last cached one keeps its own."""
+    c = Batch([1, 2], [64, 33], seed=12)
+    c.table = c.table[:, :4].contiguous()
+    c.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+    k0, v0 = c.k_cache.clone(), c.v_cache.clone()
+    q_out = torch.full_like(c.q, 7.0)
+    kv_cache.kv_append(c.k_cache, c.v_cache, c.k, c.v, c.table, c.lens, c.cu_q, q=c.q, q_out=q_out)
+    assert kv_cache.kv_status(0, clear=True) == kv_cache.BAD_LENGTH
+    assert (q_out[0] == 7.0).all() and torch.equal(q_out[1:], c.q[1:])
+    for j in (31, 32):
+        k0[int(c.table[1, j // 16]), j % 16], v0[int(c.table[1, j // 16]), j % 16] = c.k[j - 30], c.v[j - 30]
+    assert torch.equal(c.k_cache, k0) and torch.equal(c.v_cache, v0)

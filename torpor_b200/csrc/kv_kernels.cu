@@ -145,7 +145,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
                 SeqRows r;
                 const uint32_t wrong = read_rows(a.batch, b, a.batch.tokens, a.cache.page_size, r);
                 if (wrong) atomicOr(&g_kv_status, wrong);
-                j = (int)tok < r.first + r.n ? r.len - r.n + ((int)tok - r.first) : -1;
+                // a length that had to be changed says nothing about where a row goes: another token lies there
+                j = (int)tok < r.first + r.n && !(wrong & TSW_KV_BAD_LENGTH) ? r.len - r.n + ((int)tok - r.first) : -1;
                 if (j >= 0) {
                     page = ((const int*)a.batch.page_table)[(uint64_t)b * a.batch.table_stride + j / (int)a.cache.page_size];
                     at = j % (int)a.cache.page_size;
