@@ -48,3 +48,18 @@ def test_tile_numbers_stay_within_32_bits(tmp_path):
 
 def test_a_row_sees_all_keys_its_mask_leaves_it(tmp_path):
     run(build("kv_seen_probe", tmp_path))
+
+
+def test_no_report_is_lost_between_a_look_at_the_status_and_its_clearing(tmp_path):
+    if not os.path.exists("/usr/local/cuda/include/cuda_runtime.h"):
+        pytest.skip("CUDA headers not present")
+    csrc = os.path.join(os.path.dirname(HERE), "torpor_b200", "csrc")
+    exe = str(tmp_path / "kv_status_probe")
+    r = subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-pthread", "-o", exe, os.path.join(HERE, "kv_status_probe.cpp"),
+                        *(os.path.join(csrc, f) for f in ("engine.cpp", "engine_swap.cpp", "engine_share.cpp", "pool.cpp", "evictor.cpp", "scheduler.cpp",
+                                                          "controller.cpp", "kv_cache.cpp")),
+                        "-I/usr/local/cuda/include", "-L/usr/local/cuda/lib64", "-lcudart", "-lrt", "-ldl"], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-3000:]
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60,
+                       env=dict(os.environ, LD_LIBRARY_PATH="/usr/local/cuda/lib64:" + os.environ.get("LD_LIBRARY_PATH", "")))
+    assert r.returncode == 0 and r.stdout == "ok 4096\n", (r.stdout, r.stderr)

@@ -299,7 +299,7 @@ int tsw_kv_status(int device, void* stream, uint32_t* status, int clear) {
         TSW_CUDA(cudaMemcpyAsync(&seen, word, sizeof(seen), cudaMemcpyDeviceToHost, s));
         TSW_CUDA(cudaStreamSynchronize(s));
         if (clear && seen) {
-            TSW_CUDA(cudaMemsetAsync(word, 0, sizeof(seen), s));
+            TSW_CUDA(launch_kv_status_clear(word, seen, s));      // what was seen, and nothing that came since
             TSW_CUDA(cudaStreamSynchronize(s));
         }
         *status = seen;

@@ -263,6 +263,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) attention_rows_kernel(const __
     if (a.lse && lane == 0) ((float*)a.lse)[row] = total == 0.f ? -INFINITY : top + logf(total);
 }
 
+__global__ void status_clear_kernel(uint32_t* word, uint32_t bits) { atomicAnd(word, ~bits); }
+
 // Launch with an error of its own: the runtime's last error may be another call's.
 template <typename... P, typename... A>
 cudaError_t launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, const A&... args) {
@@ -290,6 +292,10 @@ cudaError_t launch_append_vec(const tsw_kv_append_args& a, int vec, dim3 grid, u
 }
 
 }  // namespace
+
+cudaError_t launch_kv_status_clear(uint32_t* word, uint32_t bits, cudaStream_t stream) {
+    return launch(status_clear_kernel, 1, 1, 0, stream, word, bits);
+}
 
 cudaError_t launch_kv_append(const tsw_kv_append_args& a, int device_sms, cudaStream_t stream) {
     // The widest vector that every address, stride and pair distance is a multiple of.

@@ -13,6 +13,7 @@ namespace tsw {
 cudaError_t launch_kv_append(const tsw_kv_append_args& a, int device_sms, cudaStream_t stream);
 cudaError_t launch_prefix_attention_rows(const tsw_prefix_attention_args& a, cudaStream_t stream);
 cudaError_t kv_status_symbol(uint32_t** word);   // address on the current device
+cudaError_t launch_kv_status_clear(uint32_t* word, uint32_t bits, cudaStream_t stream);
 
 }  // namespace tsw
 #endif
