@@ -160,6 +160,10 @@ class SwapServer:
         self.evictions = 0
         self.local_hits = 0
         self.completed = 0
+        self.decoded = 0                            # of them, requests that ran their attention
+        # requests whose attention reported something (kv_cache.kv_status): dict(func, gpu, status).  They are not completed ones.
+        # The word is one to a device: with several engines on it, the first request to end is charged.
+        self.faults: List[dict] = []
         # functions of the language-model sets run the attention of decode_tokens generated tokens; 0 = the constant of every other
         self.decode_tokens, self.prompt_tokens = decode_tokens, prompt_tokens
         self.decode: Dict[str, tuple] = {}          # func -> (PromptDecode, its model, client address of its workspace block)
@@ -210,6 +214,11 @@ class SwapServer:
         done = torch.cuda.Event()
         done.record(self.streams[g])
         return done
+
+    def _decode_status(self, g: int) -> int:
+        """What the kernels of the decode that has just ended on GPU g reported (0 = nothing)."""
+        from . import kv_cache
+        return kv_cache.kv_status(self.devices[g], self.streams[g].cuda_stream, clear=True)
 
     def _carry_out(self, events, t_arrival):
         """Executor side of the signals of one controller event."""
@@ -264,7 +273,12 @@ class SwapServer:
                 st["until"] = now + EXEC_MS.get(self.arch[st["func"]], 10.0) / 1e3
             if st["kind"] == "exec" and (st["event"].query() if st.get("event") is not None else now >= st["until"]):
                 self.state[g] = dict(kind="idle")
-                self.completed += 1
+                status = self._decode_status(g) if st.get("event") is not None else 0
+                if status:
+                    self.faults.append(dict(func=st["func"], gpu=g, status=status))
+                else:
+                    self.completed += 1
+                    self.decoded += st.get("event") is not None
                 events = self.ctrl.complete(g)                           # replica registered, pin released, queue served
                 started = any(e[0] == "S" and e[2] == SIGNAL_EXECUTE for e in events)
                 self._carry_out(events, self.arrivals.popleft() if started and self.arrivals else now)
@@ -300,7 +314,6 @@ def run_stream(n_gpus: int, n_models: int, rate: float, duration_s: float, cap_b
             k += 1
         srv.poll()
     wall = time.perf_counter() - start
-    decoded = sum(1 for p in picks if f"fn{int(p)}" in srv.decode)
     ms = np.array([s["ms"] for s in srv.swaps]) if srv.swaps else np.zeros(1)
     by = np.array([s["bytes"] for s in srv.swaps], dtype=np.float64) if srv.swaps else np.zeros(1)
     rel = np.array([s["t"] - start for s in srv.swaps]) if srv.swaps else np.zeros(1)
@@ -328,7 +341,7 @@ def run_stream(n_gpus: int, n_models: int, rate: float, duration_s: float, cap_b
         "per_swap_gbs_p50": float(np.percentile(by / (ms / 1e3) / 1e9, 50)) if srv.swaps else 0.0,
         "exec_model": "GPU occupancy per request modelled as a constant per architecture (EXEC_MS); inference not run" if not srv.decode else
                       f"attention of {decode_tokens} generated tokens behind a prompt of {prompt_tokens} for the language-model sets; others EXEC_MS",
-        "requests_decoded": decoded,
+        "requests_decoded": srv.decoded, "requests_failed": len(srv.faults),
     }
     srv.close()
     return out
