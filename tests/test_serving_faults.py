@@ -112,3 +112,32 @@ def test_functions_that_do_not_decode_are_not_asked(world, monkeypatch):
     finish(srv)
     assert srv.completed == 1 and srv.decoded == 0 and not srv.faults
     srv.close()
+
+
+def test_the_time_of_a_swap_does_not_hold_the_enqueueing_of_its_decode(world):
+    """A request is 2 layers of 2 calls a step, 100 us of host time each: 20 ms, behind swaps of 3 ms."""
+    srv = server()
+    layers = W.ATTENTION[ARCH].layers
+    for i in range(6):
+        srv.submit(f"fn{i % 3}", world.now)
+        finish(srv)
+    assert srv.completed == 6 and world.calls == 6 * STEPS * layers * 2
+    assert len(srv.swaps) >= 3
+    slice_ms = 2 * world.call_s * 1e3
+    for s in srv.swaps:
+        assert world.swap_s * 1e3 <= s["ms"] <= world.swap_s * 1e3 + slice_ms + 0.1, s
+    srv.close()
+
+
+def test_a_decode_on_one_gpu_does_not_hold_up_the_look_at_another(world):
+    srv = server(n_gpus=3, functions=9, cap=150 << 20)
+    for i in range(18):
+        srv.submit(f"fn{i % 9}", world.now)
+        for _ in range(7):
+            srv.poll()
+    finish(srv)
+    assert srv.completed == srv.decoded == 18 and len(srv.swaps) >= 6
+    slice_ms = 2 * world.call_s * 1e3
+    for s in srv.swaps:                       # each GPU's slice lies between two looks at the same one
+        assert s["ms"] <= world.swap_s * 1e3 + 3 * slice_ms + 0.1, s
+    srv.close()

@@ -117,9 +117,9 @@ class PromptDecode:
         x.workspace, x.workspace_bytes = base + o["workspace"], self.workspace_bytes
         return x
 
-    def enqueue(self, engine: MemoryManager, func: str, model: "W.LoadedModel", block: int, stream: int) -> None:
-        """Everything of one request onto ``stream`` (a cudaStream_t).  ``model``: the function as its cold start left it;
-        ``block``: client address of a workspace block of ``block_bytes``."""
+    def calls(self, engine: MemoryManager, func: str, model: "W.LoadedModel", block: int, stream: int):
+        """Everything of one request onto ``stream`` (a cudaStream_t), a layer of a step each time the generator is asked on.
+        ``model``: the function as its cold start left it; ``block``: client address of a workspace block of ``block_bytes``."""
         at = {t.name: model.tensor_vaddr[i] for i, t in enumerate(model.ws.tensors) if ".prompt." in t.name}
         prompt = lambda l, what: at[f"model.layers.{l}.prompt.{what}"]
         check(engine.cudaMemcpyAsyncBackendHtoD(block, self.image, stream, False, func))
@@ -127,6 +127,11 @@ class PromptDecode:
             for l in range(self.shape.layers):
                 engine.kv_append(func, self._append(block, l, step), stream)
                 engine.prefix_attention(func, self._attention(block, prompt, l, step), stream)
+                yield
+
+    def enqueue(self, engine: MemoryManager, func: str, model: "W.LoadedModel", block: int, stream: int) -> None:
+        """All of ``calls`` at once."""
+        collections.deque(self.calls(engine, func, model, block, stream), maxlen=0)
 
 
 class SwapServer:
@@ -204,16 +209,19 @@ class SwapServer:
             self.decode[func] = (decode, model, model.workspace_vaddr[1])
         self._carry_out(self.ctrl.complete(g), time.perf_counter())      # registers the replica; may unload others
 
-    def _execute(self, g: int, func: str):
-        """Start the function's work on GPU g: an event to wait for, or None (modelled as a constant)."""
+    def _work(self, g: int, func: str):
+        """The function's calls on GPU g, a layer at a time, or None (modelled as a constant)."""
         if func not in self.decode:
             return None
-        import torch
         decode, model, block = self.decode[func]
-        decode.enqueue(self.engines[g], func, model, block, self.streams[g].cuda_stream)
-        done = torch.cuda.Event()
-        done.record(self.streams[g])
-        return done
+        return decode.calls(self.engines[g], func, model, block, self.streams[g].cuda_stream)
+
+    def _advance(self, g: int, st: dict) -> None:
+        """Enqueue one layer of the work on GPU g; behind the last one an event to wait for."""
+        if next(st["work"], self) is self:
+            import torch
+            st["work"], st["event"] = None, torch.cuda.Event()
+            st["event"].record(self.streams[g])
 
     def _decode_status(self, g: int) -> int:
         """What the kernels of the decode that has just ended on GPU g reported (0 = nothing)."""
@@ -243,7 +251,7 @@ class SwapServer:
                     else:
                         self.engines[g].swap_in(func, src)
             elif sig == SIGNAL_EXECUTE:
-                st = dict(func=func, t_arrival=t_arrival, event=self._execute(g, func))
+                st = dict(func=func, t_arrival=t_arrival, work=self._work(g, func), event=None)
                 if self.pending[g] is None:
                     self.local_hits += 1
                     st.update(kind="exec", until=time.perf_counter() + EXEC_MS.get(self.arch[func], 10.0) / 1e3)
@@ -262,23 +270,26 @@ class SwapServer:
         return True
 
     def poll(self):
-        """Advance every GPU: finished swaps start executing, finished executions complete."""
-        now = time.perf_counter()
+        """Advance every GPU: finished swaps start executing, finished executions complete.  A decode is enqueued a layer to a
+        poll, before its swap has ended as well as after: what a poll finds, and when, does not depend on how long a request's
+        calls take the host."""
         for g in range(self.n):
-            st = self.state[g]
+            st, now = self.state[g], time.perf_counter()
             if st["kind"] == "swap" and self.engines[g].poll_ready(st["func"]) == 0:
                 self.swaps.append(dict(func=st["func"], gpu=g, src=st["src"], bytes=self.nbytes[st["func"]],
                                        ms=(now - st["t_signal"]) * 1e3, t=st["t_signal"], links=st["links"]))
                 st["kind"] = "exec"
                 st["until"] = now + EXEC_MS.get(self.arch[st["func"]], 10.0) / 1e3
-            if st["kind"] == "exec" and (st["event"].query() if st.get("event") is not None else now >= st["until"]):
+            if st.get("work") is not None:
+                self._advance(g, st)
+            elif st["kind"] == "exec" and (st["event"].query() if st["event"] is not None else now >= st["until"]):
                 self.state[g] = dict(kind="idle")
-                status = self._decode_status(g) if st.get("event") is not None else 0
+                status = self._decode_status(g) if st["event"] is not None else 0
                 if status:
                     self.faults.append(dict(func=st["func"], gpu=g, status=status))
                 else:
                     self.completed += 1
-                    self.decoded += st.get("event") is not None
+                    self.decoded += st["event"] is not None
                 events = self.ctrl.complete(g)                           # replica registered, pin released, queue served
                 started = any(e[0] == "S" and e[2] == SIGNAL_EXECUTE for e in events)
                 self._carry_out(events, self.arrivals.popleft() if started and self.arrivals else now)
