@@ -141,3 +141,11 @@ def test_a_decode_on_one_gpu_does_not_hold_up_the_look_at_another(world):
     for s in srv.swaps:                       # each GPU's slice lies between two looks at the same one
         assert s["ms"] <= world.swap_s * 1e3 + 3 * slice_ms + 0.1, s
     srv.close()
+
+
+def test_a_stream_of_unknown_architectures_has_made_no_engine(built, monkeypatch):
+    made = []
+    monkeypatch.setattr(serving, "MemoryManager", lambda *a, **kw: made.append(a))
+    with pytest.raises(KeyError):
+        serving.run_stream(n_gpus=1, n_models=2, rate=10.0, duration_s=0.1, cap_bytes=1 << 28, archs=("no_such_set",), devices=[-1])
+    assert not made

@@ -134,6 +134,16 @@ class PromptDecode:
         collections.deque(self.calls(engine, func, model, block, stream), maxlen=0)
 
 
+def decodes(arch: str, decode_tokens: int) -> bool:
+    return decode_tokens > 0 and arch in W.ATTENTION
+
+
+def served_set(arch: str, decode_tokens: int, prompt_tokens: int, seed: Optional[int] = None) -> "W.WeightSet":
+    """The weights of a function of this architecture, with its prompt when it decodes."""
+    ws = W.weight_set(arch, seed=seed)
+    return W.with_prompt(ws, arch, prompt_tokens) if decodes(arch, decode_tokens) else ws
+
+
 class SwapServer:
     """N engines under the library's controller (``tsw_ctrl_*``): this class only carries out the
     signals the controller sends -- unload, load (from the host store or a replica), execute -- on
@@ -187,12 +197,11 @@ class SwapServer:
         repo_reset()
 
     def decodes(self, arch: str) -> bool:
-        return self.decode_tokens > 0 and arch in W.ATTENTION
+        return decodes(arch, self.decode_tokens)
 
     def weight_set(self, arch: str, seed: Optional[int] = None) -> "W.WeightSet":
         """What a function of this architecture brings along: its weights, and its prompt when it decodes."""
-        ws = W.weight_set(arch, seed=seed)
-        return W.with_prompt(ws, arch, self.prompt_tokens) if self.decodes(arch) else ws
+        return served_set(arch, self.decode_tokens, self.prompt_tokens, seed)
 
     # ---- ExecuteAfterLoad (controller.hpp:141-162, 223-227): round-robin placement, load once
     def cold_start(self, func: str, arch: str, seed: int, tensor_data=None):
@@ -304,10 +313,10 @@ def run_stream(n_gpus: int, n_models: int, rate: float, duration_s: float, cap_b
                shard_min_bytes: int = 0, pcie_pairs=None, nvlink=None, decode_tokens: int = 0, prompt_tokens: int = 1024) -> dict:
     """The mixed serverless stream: ``n_models`` functions, Zipf popularity, Poisson arrivals."""
     arch_of, times, picks = W.mixed_stream(seed=seed, n_models=n_models, rate=rate, duration_s=duration_s, archs=archs)
+    store = sum(W.host_store_bytes(served_set(a, decode_tokens, prompt_tokens)) for a in arch_of)      # refuses unknown sets before any engine
     srv = SwapServer(n_gpus, cap_bytes, evict_policy=evict_policy, host_arena_bytes=0, devices=devices,
                      shard_min_bytes=shard_min_bytes, pcie_pairs=pcie_pairs, nvlink=nvlink, decode_tokens=decode_tokens,
                      prompt_tokens=prompt_tokens)
-    store = sum(W.host_store_bytes(srv.weight_set(a)) for a in arch_of)
     t0 = time.time()
     for i, a in enumerate(arch_of):
         ws = srv.weight_set(a)
