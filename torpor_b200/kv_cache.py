@@ -9,7 +9,8 @@ pages, often among the function's parameters, so that a swap-in brings it along 
 * ``prefix_attention`` -- attention of the new tokens over the shared prefix and their sequence's pages
 
 Tensors are torch tensors on one CUDA device; the calls run on that device's current stream, allocate only
-what they return (and a workspace, from torch's allocator), and may be captured into a graph.
+what they return (and a workspace, from torch's allocator), and may be captured into a graph.  They serve: there is
+no backward pass, and operands that require a gradient are refused while gradients are recorded.
 ``MemoryManager.kv_append`` and ``MemoryManager.prefix_attention`` are the same on a function's own
 client addresses.
 """
@@ -83,6 +84,13 @@ def _batch(page_table, seq_lens, cu_q, tokens: int, device) -> _cabi.KvBatch:
     return _cabi.KvBatch(page_table.data_ptr(), seq_lens.data_ptr(), cu_q.data_ptr(), n, width, page_table.stride(0), tokens)
 
 
+def _no_gradients(call: str, *tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{call} has no backward pass: call it under torch.no_grad(), or detach what requires a gradient")
+
+
 def _dtype(t: torch.Tensor, call: str) -> int:
     if t.device.type != "cuda":
         raise ValueError(f"{call} needs CUDA tensors: there is no CPU path")
@@ -111,6 +119,7 @@ def kv_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: 
     them; own token j goes to page ``page_table[b, j // page_size]``.  ``inv_freq`` (float64, one per pair;
     ``rope_frequencies``) rotates the first ``2 * len(inv_freq)`` elements of each key and query head by
     ``(position_offset + j) * inv_freq``; ``interleaved`` pairs elements (2c, 2c + 1) instead of halves."""
+    _no_gradients("kv_append", k_cache, v_cache, k, v, q, q_out, inv_freq)
     code = _dtype(k, "kv_append")
     device, dtype = k.device, k.dtype
     a = _cabi.KvAppendArgs()
@@ -163,6 +172,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     and -inf; rows that belong to no sequence are left as they were (undefined where the result is made here).
     ``workspace``: a uint8 tensor of at least ``prefix_attention_workspace`` bytes, 256-byte aligned; default: taken from torch's
     allocator for this call."""
+    _no_gradients("prefix_attention", q, k_cache, v_cache, prefix_k, prefix_v, out)
     code = _dtype(q, "prefix_attention")
     device, dtype = q.device, q.dtype
     a = _cabi.PrefixAttentionArgs()
