@@ -50,3 +50,20 @@ def test_they_are_taken_where_no_gradient_is_recorded(built, call, name):
         call(o)
     with torch.no_grad():
         assert torch.equal(call(o), want)
+
+
+@pytest.mark.gpu
+def test_what_is_written_is_seen_by_graphs_that_kept_it(built):
+    w = torch.ones(1, 2, 64, dtype=torch.float16, device="cuda", requires_grad=True)
+    for call, name in ((append, "k_cache"), (append, "v_cache"), (append, "q_out"), (attend, "out")):
+        o = operands("cuda")
+        before = {n: t._version for n, t in o.items()}
+        loss = (o[name][:1].reshape(-1, 2, 64)[:1] * w).sum()
+        call(o)
+        written = {"k_cache", "v_cache", "q_out"} if call is append else {"out"}
+        assert {n for n, t in o.items() if t._version != before[n]} == written
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        o = operands("cuda")
+        append(o), attend(o)                                          # tensors without a version

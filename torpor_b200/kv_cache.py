@@ -100,6 +100,11 @@ def _dtype(t: torch.Tensor, call: str) -> int:
     return code
 
 
+# torch is told what was written behind its back: a graph that has kept one of these for its backward pass then says so
+# instead of using the new values.
+_written = torch.autograd.graph.increment_version
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # without a Stream object around it
 
 
@@ -152,6 +157,7 @@ def kv_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: 
     a.dtype, a.kv_heads, a.head_dim = code, heads, dim
     if tokens:
         check(_cabi.lib().tsw_kv_append(device.index, C.byref(a), _stream(device)))
+        _written((k_cache, v_cache) if q_out is None else (k_cache, v_cache, q_out))
     return q_out
 
 
@@ -226,6 +232,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         if workspace is not None:
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
         check(L.tsw_prefix_attention(device.index, C.byref(a), _stream(device)))
+        _written((out,))
     return (out, lse) if return_lse else out
 
 
