@@ -212,3 +212,28 @@ def test_append_beyond_the_table_overwrites_nothing(lens):
     for j in (31, 32):
         k0[int(c.table[1, j // 16]), j % 16], v0[int(c.table[1, j // 16]), j % 16] = c.k[j - 30], c.v[j - 30]
     assert torch.equal(c.k_cache, k0) and torch.equal(c.v_cache, v0)
+
+
+@pytest.mark.parametrize("where", ["prefix", "own"])
+def test_the_row_kernel_sums_more_keys_than_32_bits_count_one_by_one(where):
+    """2^24 + 2^20 equal scores, values 1: the result is 1.  Sums of up to 2^15 ones are exact, and so are those of their sums."""
+    n, ps = (1 << 24) + (1 << 20) + 5, 1 << 20
+    table = torch.zeros(-(-n // ps), dtype=torch.int32, device="cuda")
+    k, v = torch.zeros(1, ps, 1, 2, dtype=torch.float16, device="cuda"), torch.ones(1, ps, 1, 2, dtype=torch.float16, device="cuda")
+    q, cu = torch.randn(1, 1, 2, device="cuda").half(), torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    if where == "prefix":
+        none = torch.zeros(1, 0, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+        out, lse = kv_cache.prefix_attention(q, k, v, *none, cu, prefix_table=table, prefix_len=n, return_lse=True)
+    else:
+        out, lse = kv_cache.prefix_attention(q, k, v, table[None], torch.tensor([n], dtype=torch.int32, device="cuda"), cu, return_lse=True)
+    assert (out == 1.0).all()
+    assert abs(lse.item() - math.log(n)) <= 2.0 ** -22 * 17
+
+
+@pytest.mark.parametrize("dim", [200, 512, 50])
+def test_the_row_kernel_joins_its_sums(dim):
+    """Over the borders of its partial sums, with maxima that move on both sides of them."""
+    c = Batch([1, 2], [40000, 33000], dim=dim, prefix=32768 * 2 + 17, seed=15, page_size=512)
+    out, lse = kv_cache.prefix_attention(c.q, c.k_cache, c.v_cache, c.table, c.lens, c.cu_q, max_q=2, prefix_table=c.prefix_table, prefix_len=c.prefix,
+                                         return_lse=True)
+    c.check(out, lse)

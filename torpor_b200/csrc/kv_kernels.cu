@@ -190,6 +190,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
 // against 71 us of the tile kernel.
 constexpr int kRowWarps = 4;
 constexpr int kRowMaxDim = 512;
+constexpr int kRowFold = 1024;
 
 template <typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) attention_rows_kernel(const __grid_constant__ tsw_prefix_attention_args a) {
@@ -213,6 +214,12 @@ __global__ void __launch_bounds__(32 * kRowWarps) attention_rows_kernel(const __
     float acc[kRowMaxDim / 32];
 #pragma unroll
     for (int i = 0; i < kRowMaxDim / 32; ++i) acc[i] = 0.f;
+    // A sum of 2^24 equal weights takes up no more of them in 32 bits.  So the sums go over kRowFold rounds at a time, and those over
+    // the rest of the keys: 2^15 additions and 2^16.
+    float all[kRowMaxDim / 32], all_total = 0.f;
+#pragma unroll
+    for (int i = 0; i < kRowMaxDim / 32; ++i) all[i] = 0.f;
+    int rounds = 0;
     float top = -INFINITY, total = 0.f;
     for (int part = 0; part < 2; ++part) {
         const tsw_kv_pages& pg = part ? a.cache : a.prefix;
@@ -239,9 +246,23 @@ __global__ void __launch_bounds__(32 * kRowWarps) attention_rows_kernel(const __
             const float keep = expf(top - base);
             const float e = expf(s - base);
             total = total * keep + warp_sum(e);
+            all_total *= keep;
             top = new_top;
 #pragma unroll
-            for (int i = 0; i < kRowMaxDim / 32; ++i) acc[i] *= keep;
+            for (int i = 0; i < kRowMaxDim / 32; ++i) {
+                acc[i] *= keep;
+                all[i] *= keep;
+            }
+            if (++rounds == kRowFold) {
+                rounds = 0;
+                all_total += total;
+                total = 0.f;
+#pragma unroll
+                for (int i = 0; i < kRowMaxDim / 32; ++i) {
+                    all[i] += acc[i];
+                    acc[i] = 0.f;
+                }
+            }
             const int m = min(32, end - k0);
             for (int i = 0; i < m; ++i) {
                 const float w = __shfl_sync(~0u, e, i);
@@ -255,11 +276,12 @@ __global__ void __launch_bounds__(32 * kRowWarps) attention_rows_kernel(const __
             }
         }
     }
+    total += all_total;
     const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;   // a row that saw nothing: zeros; NaN stays
     T* out = (T*)(a.out + tok * a.out_token_stride + head * a.out_head_stride);
 #pragma unroll
     for (int i = 0; i < kRowMaxDim / 32; ++i)
-        if (lane + 32 * i < dim) out[lane + 32 * i] = from_float<T>(acc[i] * inv);
+        if (lane + 32 * i < dim) out[lane + 32 * i] = from_float<T>((acc[i] + all[i]) * inv);
     if (a.lse && lane == 0) ((float*)a.lse)[row] = total == 0.f ? -INFINITY : top + logf(total);
 }
 
