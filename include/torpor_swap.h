@@ -416,7 +416,8 @@ int tsw_kv_status(int device, void* stream, uint32_t* status, int clear);
  * `func` and is translated as the executor translates a kernel's arguments (cuda_server.hpp:1265-1268);
  * each operand must lie inside one block of the function (TSW_ERR_NOT_FOUND otherwise).  Parameters
  * that are still being swapped in are waited for on the stream, as in tsw_translate_async, and are recorded as
- * accessed.  TSW_ERR_STATE when a block is not on the engine's GPU. */
+ * accessed.  TSW_ERR_STATE when a block is not on the engine's GPU, and on a stream that is being captured: the next swap-in
+ * may place the blocks elsewhere, and a graph would keep where they lie now. */
 int tsw_func_kv_append(tsw_engine* e, const char* func, const tsw_kv_append_args* args, void* stream);
 int tsw_func_prefix_attention(tsw_engine* e, const char* func, const tsw_prefix_attention_args* args, void* stream);
 

@@ -237,3 +237,35 @@ def test_the_row_kernel_joins_its_sums(dim):
     out, lse = kv_cache.prefix_attention(c.q, c.k_cache, c.v_cache, c.table, c.lens, c.cu_q, max_q=2, prefix_table=c.prefix_table, prefix_len=c.prefix,
                                          return_lse=True)
     c.check(out, lse)
+
+
+def test_calls_on_a_functions_memory_cannot_be_captured(built):
+    """Its blocks move with every swap-in; a replay would go to where they lay."""
+    from torpor_b200 import serving
+    from torpor_b200 import workloads as W
+    from torpor_b200.memory_manager import MemoryManager, SwapError, repo_reset
+    repo_reset()
+    ws = W.with_prompt(W.weight_set("llama_tiny", seed=5), "llama_tiny", 20)
+    decode = serving.PromptDecode("llama_tiny", 20, 2)
+    with MemoryManager(0, device=0) as eng:
+        model = W.cold_start(eng, "f", ws, workspace_blocks=(W.SMALL_BLOCK, decode.block_bytes))
+        block = model.workspace_vaddr[1]
+        at = {t.name: model.tensor_vaddr[i] for i, t in enumerate(ws.tensors)}
+        append = decode._append(block, 0, 0)
+        attention = decode._attention(block, lambda l, what: at[f"model.layers.{l}.prompt.{what}"], 0, 0)
+        stream = torch.cuda.Stream()
+        decode.enqueue(eng, "f", model, block, stream.cuda_stream)
+        stream.synchronize()
+        for call, args in ((eng.kv_append, append), (eng.prefix_attention, attention)):
+            graph, x = torch.cuda.CUDAGraph(), torch.zeros(1, device="cuda")
+            with torch.cuda.graph(graph, stream=stream):
+                with pytest.raises(SwapError) as e:
+                    call("f", args, stream.cuda_stream)
+                x += 1
+            assert e.value.code == _cabi.ERR_STATE
+            graph.replay()
+            torch.cuda.synchronize()
+            assert x.item() == 1
+            call("f", args, stream.cuda_stream)
+        stream.synchronize()
+    repo_reset()

@@ -234,6 +234,14 @@ int engine_ok(tsw_engine* e, const char* func, const void* args) {
     return TSW_OK;
 }
 
+// Blocks lie elsewhere after the next swap-in: a graph would keep the addresses of this one, and write to what lies there by then.
+int not_captured(void* stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    TSW_CUDA(cudaStreamIsCapturing((cudaStream_t)stream, &status));
+    if (status != cudaStreamCaptureStatusNone) return fail(TSW_ERR_STATE, "a function's addresses hold until its next swap: the call cannot be captured");
+    return TSW_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -314,6 +322,7 @@ int tsw_func_kv_append(tsw_engine* e, const char* func, const tsw_kv_append_args
         tsw_kv_append_args a = *args;
         const uint64_t row = 2ull * a.head_dim;
         const DeviceGuard guard(e->cfg.device);
+        CHECK(not_captured(stream));
         Lock g1(repo().mu);
         Lock g2(e->mu);
         CHECK(operand_pages(e, func, a.cache, row, a.kv_heads, stream));
@@ -338,6 +347,7 @@ int tsw_func_prefix_attention(tsw_engine* e, const char* func, const tsw_prefix_
         tsw_prefix_attention_args a = *args;
         const uint64_t row = 2ull * a.head_dim;
         const DeviceGuard guard(e->cfg.device);
+        CHECK(not_captured(stream));
         Lock g1(repo().mu);
         Lock g2(e->mu);
         CHECK(operand_pages(e, func, a.cache, row, a.kv_heads, stream));
