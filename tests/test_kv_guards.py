@@ -63,3 +63,7 @@ def test_no_report_is_lost_between_a_look_at_the_status_and_its_clearing(tmp_pat
     r = subprocess.run([exe], capture_output=True, text=True, timeout=60,
                        env=dict(os.environ, LD_LIBRARY_PATH="/usr/local/cuda/lib64:" + os.environ.get("LD_LIBRARY_PATH", "")))
     assert r.returncode == 0 and r.stdout == "ok 4096\n", (r.stdout, r.stderr)
+
+
+def test_a_workspace_holds_the_lists_there_are(tmp_path):
+    run(build("kv_workspace_probe", tmp_path))

@@ -17,7 +17,7 @@ struct AttentionLayout {
     uint32_t prefix_pair, own_pair;   // the list is dealt to the two streams of a CTA together
     uint32_t part_rows;       // rows of a partial result that is not an item's first
     // Workspace, in bytes from its start.  A result that is an item's first range lies by row
-    // ([list][token][head]); the ranges that continue an item (at most one per stream and list) lie by stream.
+    // ([list][token][head], one list without a prefix); the ranges that continue an item (at most one per stream and list) lie by stream.
     uint64_t own_base;        // uint32 [batch + 2]: tiles in front of each sequence's; own total; prefix total
     uint64_t home_ml, home_o; // float2, float [head_dim]
     uint64_t part_ml, part_o;

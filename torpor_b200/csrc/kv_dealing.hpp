@@ -140,7 +140,8 @@ inline bool attention_layout(const tsw_prefix_attention_args& a, int sms, Attent
         at += (bytes + 255) & ~255ull;
         return here;
     };
-    const uint64_t rows = 2ull * a.batch.tokens * a.q_heads, parts = 4ull * w->ctas * w->part_rows;
+    // Results of one list, and of two behind a prefix.
+    const uint64_t lists = a.prefix_len ? 2 : 1, rows = lists * a.batch.tokens * a.q_heads, parts = lists * 2 * w->ctas * w->part_rows;
     w->own_base = part(4ull * (a.batch.batch + 2));
     w->home_ml = part(8 * rows);
     w->home_o = part(4 * rows * a.head_dim);
@@ -469,9 +470,10 @@ TSW_HD Parts own_parts(const Deal& d, const SeqRows& r, int tok, int kv_head, ui
     p.last = range_of(x + seen - 1, total, n);
     return p;
 }
-TSW_HD uint64_t home_index(const Deal& d, int list, uint64_t row, uint32_t q_heads) { return (uint64_t)list * d.batch.tokens * q_heads + row; }
+TSW_HD int list_place(const Deal& d, int list) { return d.prefix_len ? list : 0; }      // without a prefix the own list is the only one
+TSW_HD uint64_t home_index(const Deal& d, int list, uint64_t row, uint32_t q_heads) { return (uint64_t)list_place(d, list) * d.batch.tokens * q_heads + row; }
 TSW_HD uint64_t part_index(const Deal& d, int list, uint32_t place, uint32_t row_in_tile) {
-    return ((uint64_t)list * 2 * d.w.ctas + place) * d.w.part_rows + row_in_tile;
+    return ((uint64_t)list_place(d, list) * 2 * d.w.ctas + place) * d.w.part_rows + row_in_tile;
 }
 
 }  // namespace tsw
