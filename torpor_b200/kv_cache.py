@@ -84,11 +84,11 @@ def _batch(page_table, seq_lens, cu_q, tokens: int, device) -> _cabi.KvBatch:
     return _cabi.KvBatch(page_table.data_ptr(), seq_lens.data_ptr(), cu_q.data_ptr(), n, width, page_table.stride(0), tokens)
 
 
-def _no_gradients(call: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError(f"{call} has no backward pass: call it under torch.no_grad(), or detach what requires a gradient")
+_records = torch.is_grad_enabled
+
+
+def _refuse_gradients(call: str) -> None:
+    raise ValueError(f"{call} has no backward pass: call it under torch.no_grad(), or detach what requires a gradient")
 
 
 def _dtype(t: torch.Tensor, call: str) -> int:
@@ -102,8 +102,7 @@ def _dtype(t: torch.Tensor, call: str) -> int:
 
 # torch is told what was written behind its back: a graph that has kept one of these for its backward pass then says so
 # instead of using the new values.
-_written = torch.autograd.graph.increment_version
-
+_written = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)      # the second wraps the first
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # without a Stream object around it
 
@@ -124,7 +123,9 @@ def kv_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: 
     them; own token j goes to page ``page_table[b, j // page_size]``.  ``inv_freq`` (float64, one per pair;
     ``rope_frequencies``) rotates the first ``2 * len(inv_freq)`` elements of each key and query head by
     ``(position_offset + j) * inv_freq``; ``interleaved`` pairs elements (2c, 2c + 1) instead of halves."""
-    _no_gradients("kv_append", k_cache, v_cache, k, v, q, q_out, inv_freq)
+    if _records() and (k_cache.requires_grad or v_cache.requires_grad or k.requires_grad or v.requires_grad or (q is not None and q.requires_grad) or
+                       (q_out is not None and q_out.requires_grad) or (inv_freq is not None and inv_freq.requires_grad)):
+        _refuse_gradients("kv_append")
     code = _dtype(k, "kv_append")
     device, dtype = k.device, k.dtype
     a = _cabi.KvAppendArgs()
@@ -178,7 +179,9 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     and -inf; rows that belong to no sequence are left as they were (undefined where the result is made here).
     ``workspace``: a uint8 tensor of at least ``prefix_attention_workspace`` bytes, 256-byte aligned; default: taken from torch's
     allocator for this call."""
-    _no_gradients("prefix_attention", q, k_cache, v_cache, prefix_k, prefix_v, out)
+    if _records() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or (prefix_k is not None and prefix_k.requires_grad) or
+                       (prefix_v is not None and prefix_v.requires_grad) or (out is not None and out.requires_grad)):
+        _refuse_gradients("prefix_attention")
     code = _dtype(q, "prefix_attention")
     device, dtype = q.device, q.dtype
     a = _cabi.PrefixAttentionArgs()
