@@ -329,8 +329,13 @@ int tsw_place_segments_static_status(int device, void* stream, uint32_t* status,
  * and everything that corresponds to them is left as it was.  All three tables are int32 in
  * device memory and are read on the device, so a captured call follows their contents on replay.
  *
- * Types: TSW_F16 and TSW_BF16, the same for all operands of a call; sums, statistics and
- * rotations are held in 32 bits or more, and each result is rounded once.  Strides are in bytes;
+ * Types: TSW_F16 and TSW_BF16, the same for all operands of a call; sums, maxima, log-sums and
+ * rotations are held in 32 bits or more, and each result is rounded once.  One thing has 16 bits: on the tensor cores a
+ * softmax weight is rounded to the operands' type before it meets its value (not before it is summed), half a step relative
+ * (2^-11 in fp16, 2^-8 in bf16: results are off by 1.3 to 1.4 times what their own rounding takes).  Calls that the
+ * tensor cores do not take -- heads of more than 128 elements or no multiple of 8, pages of no power of two, addresses
+ * or strides of no multiple of 16 bytes, scale <= 0, more than 128 query heads to a key head, a cache of no pages, 2^31 tiles or more -- run a
+ * general kernel, some 30 times slower, whose weights have 32 bits.  Strides are in bytes;
  * the elements of a head are contiguous.  Operands that are written keep their rows apart: taken by stride, each
  * dimension steps over all that the ones before it cover (TSW_ERR_INVALID otherwise).  Head h of the queries reads key head
  * h / (q_heads / kv_heads).
@@ -384,8 +389,8 @@ int tsw_kv_append(int device, const tsw_kv_append_args* args, void* stream);
  * up to its own number; with causal = 0 all own tokens of its sequence (an encoder's states, say).
  * A row that sees nothing gets zeros and a log-sum of -inf.  The prefix is read once for all
  * sequences, not once for each.  What lies in a page behind the last token is not read into any
- * result, whatever its bits.  A value that is infinite or NaN reaches every row of its own sequence in
- * the same call (for a prefix value: every row), also the rows that stand before it.
+ * result, whatever its bits.  On the tensor cores a value that is infinite or NaN may reach every row of its own sequence in
+ * the same call (for a prefix value: every row), also the rows that stand before it (a weight of zero times infinity).
  * lse, when given, receives ln(sum of exp) per row and head, float [tokens][q_heads].
  * The result is the same bit for bit on every call with the same arguments and tables.
  * workspace: tsw_prefix_attention_workspace(args) bytes of device memory, 256-byte aligned, in use until the
@@ -408,7 +413,7 @@ int tsw_prefix_attention_workspace(const tsw_prefix_attention_args* args, uint64
 int tsw_prefix_attention(int device, const tsw_prefix_attention_args* args, void* stream);
 
 /* What the two operators' kernels found wrong in device tables since the word was last cleared: a sum
- * of TSW_KV_*; 0 = nothing.  Synchronises `stream`; clear != 0 resets the word. */
+ * of TSW_KV_*; 0 = nothing.  Synchronises `stream`; clear != 0 takes back what is told, and nothing that is reported meanwhile. */
 enum { TSW_KV_BAD_PAGE = 1, TSW_KV_BAD_LENGTH = 2, TSW_KV_BAD_ROWS = 4, TSW_KV_WAIT_GAVE_UP = 8 };
 int tsw_kv_status(int device, void* stream, uint32_t* status, int clear);
 

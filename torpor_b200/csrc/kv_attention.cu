@@ -24,9 +24,10 @@
 // arithmetic is done and fetched once), two warps load keys and values page by page with TMA, two
 // threads issue the products.
 //
-// Measured: 4096 rows of 32 heads of 128 behind 16384 tokens, 1.11 ms for this kernel, 1020 TFLOP/s, the tensor
-// pipe 72 % busy (exponentials: the special function unit at 54 %); a causal prompt of 8192 tokens 0.64 ms, 859 TFLOP/s;
-// eight texts of up to 32768 tokens, 84 us, 5.8 TB/s.  Short jobs are bound by what each costs its rows beside the tiles
+// Measured, for this kernel alone and thus under ncu, cold: 4096 rows of 32 heads of 128 behind 16384 tokens, 1.80 million
+// cycles (1.12 to 1.15 ms at 1.61 to 1.56 GHz, 1020 to 990 TFLOP/s), the tensor pipe 71 % busy (exponentials: the special
+// function unit at 54 %); a causal prompt of 8192 tokens 1.16 million cycles (650 to 684 us, 845 to 803 TFLOP/s);
+// eight texts of up to 32768 tokens, 86 to 90 us, 5.6 to 5.4 TB/s.  Short jobs are bound by what each costs its rows beside the tiles
 // (queries, the wait for the last product, storing: some 2000 cycles) and by 5 us before the first key arrives.
 
 #include "kv_kernels.hpp"
@@ -735,9 +736,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
 // kernel is worked out while it still runs.
 //
 // `many`: a warp takes a token with all its heads.  Without a prefix nearly every row is complete already, and what
-// the others cost is the search that finds it so, which is then made once to a token.  A causal prompt of 8192 tokens 757 us
-// with four heads to a warp, 745 so.  Where rows have to be joined, or tokens are few, the heads go side by side: 500 rows
-// of an encoder's 22.8 us, 28.7 the other way; 32 sequences behind 2048 tokens 70.6 and 171.9.
+// the others cost is the search that finds it so, which is then made once to a token.  Where rows have to be joined, or
+// tokens are few, the heads go side by side: 500 rows of an encoder's 22.8 us, 28.7 the other way; 32 sequences behind 2048
+// tokens 70.6 and 171.9.  Without a prefix, side by side / a warp to a token, us, 32 heads of 128 in bf16, and 32 on 8:
+//   tokens                  1024          2048          4096          8192
+//   one causal text         50 / 65       93 / 99       249 / 245     730 / 712
+//   on 8 key heads          50 / 67       109 / 116     274 / 268     762 / 738
+//   texts of 128 tokens     27.8 / 29.7   39.9 / 37.9   64.5 / 56.4   105 / 87
 constexpr int kJoinThreads = 128, kJoinWarps = kJoinThreads / 32;
 constexpr uint32_t kManyTokens = 4096;
 template <typename T, int DP>

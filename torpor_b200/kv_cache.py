@@ -173,8 +173,9 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     The prefix is ``prefix_len`` tokens in the pages ``prefix_table`` (int32) of ``prefix_k`` / ``prefix_v`` (default: the cache
     itself); it is read once for the whole batch.  Rows, tables and cache are those of ``kv_append``.  A
     row sees the prefix and, with ``causal``, the own tokens up to itself; without, all own tokens of its
-    sequence (queries on an encoder's states, for one).  ``max_q`` is the most new tokens any sequence has (default:
-    the number of rows; 1 while generating).  ``scale`` defaults to ``head_dim ** -0.5``.  ``lse`` is the
+    sequence (queries on an encoder's states, for one).  ``max_q`` is the most new tokens any sequence has, or more (default:
+    the number of rows).  Give it while generating: where the rows of a key head pass 128, a bound of 1 is up to a
+    quarter faster than the default (200 sequences behind 2048 tokens 192 for 237 us).  ``scale`` defaults to ``head_dim ** -0.5``.  ``lse`` is the
     natural logarithm of the sum of exponentials, float32 [tokens, q_heads].  Rows that see nothing get zeros
     and -inf; rows that belong to no sequence are left as they were (undefined where the result is made here).
     ``workspace``: a uint8 tensor of at least ``prefix_attention_workspace`` bytes, 256-byte aligned; default: taken from torch's
