@@ -269,3 +269,40 @@ def test_calls_on_a_functions_memory_cannot_be_captured(built):
             call("f", args, stream.cuda_stream)
         stream.synchronize()
     repo_reset()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("scale", [1.0, 0.7, 5.3])
+@pytest.mark.parametrize("where", ["prefix", "own"])
+def test_scores_of_any_size_leave_finite_results(dtype, scale, where):
+    """Every 5th key has the largest score, exactly, the others one that is 2^-7 smaller (or larger, where scores are negative): sums of one
+    product, so scores are exact before the scale.  Rows whose scores lie 40 or more apart are the average of the
+    largest keys' values; all rows are averages of values between 1 and 2.  Weights rounded once, the result once: 2.01 half steps,
+    2^-12 for sums and their joining; where scores lie apart, what the others add is below e^-40 * 5."""
+    n, ps, dim, heads = 3000, 64, 64, 46
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k = torch.zeros(-(-n // ps), ps, 1, dim, dtype=dtype, device="cuda")
+    v = torch.rand(k.shape, generator=g, device="cuda").add(1).to(dtype)
+    at = torch.arange(k.shape[0] * ps, device="cuda").view(k.shape[:2])
+    big = 2.0 ** 15 if dtype is torch.float16 else 2.0 ** 60
+    k[..., 0, 0] = torch.where(at % 5 == 3, big, big * (1 - 2.0 ** -7)).to(dtype)
+    k[..., 0, 1] = torch.where(at % 5 == 3, big * (1 - 2.0 ** -7), big).to(dtype)
+    q = torch.zeros(1, heads, dim, dtype=dtype, device="cuda")
+    half = heads // 2
+    sizes = [2.0 ** (15 - i) if dtype is torch.float16 else 2.0 ** (55 - 5 * i) for i in range(half)]
+    for i, s in enumerate(sizes):
+        q[0, i, 0] = s                       # positive scores
+        q[0, half + i, 1] = -s               # negative ones: the smallest in size is the largest
+    table, cu = torch.arange(k.shape[0], dtype=torch.int32, device="cuda"), torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([n if where == "own" else 0], dtype=torch.int32, device="cuda")
+    out, lse = kv_cache.prefix_attention(q, k, v, table[None], lens, cu, max_q=1, scale=scale, return_lse=True,
+                                         **(dict(prefix_table=table, prefix_len=n) if where == "prefix" else {}))
+    out = out.double()[0]
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
+    assert (out >= 1 - 4 * u).all() and (out <= 2 + 8 * u).all()
+    vals = v.view(-1, dim)[:n].double()
+    want = vals[torch.arange(n, device="cuda") % 5 == 3].mean(0)
+    apart = torch.tensor([s * big * scale * 2.0 ** -7 >= 40 for s in sizes] * 2, device="cuda")
+    assert apart.sum() >= 10
+    assert ((out - want).abs()[apart] <= want * (2.01 * u + 2.0 ** -12) + 5 * math.exp(-40)).all()
