@@ -24,10 +24,10 @@
 // arithmetic is done and fetched once), two warps load keys and values page by page with TMA, two
 // threads issue the products.
 //
-// Measured, for this kernel alone and thus under ncu, cold: 4096 rows of 32 heads of 128 behind 16384 tokens, 1.80 million
-// cycles (1.12 to 1.15 ms at 1.61 to 1.56 GHz, 1020 to 990 TFLOP/s), the tensor pipe 71 % busy (exponentials: the special
-// function unit at 54 %); a causal prompt of 8192 tokens 1.16 million cycles (650 to 684 us, 845 to 803 TFLOP/s);
-// eight texts of up to 32768 tokens, 86 to 90 us, 5.6 to 5.4 TB/s.  Short jobs are bound by what each costs its rows beside the tiles
+// Measured, for this kernel alone and thus under ncu, cold: 4096 rows of 32 heads of 128 behind 16384 tokens, 1.88 million
+// cycles (1.21 ms at 1.56 GHz, 942 TFLOP/s), the tensor pipe 70 % busy (exponentials: the special function unit at
+// 53 %); a causal prompt of 8192 tokens 1.17 million cycles (690 us, 796 TFLOP/s); eight texts of up to 32768 tokens, 86 to
+// 89 us, 5.6 to 5.4 TB/s.  Short jobs are bound by what each costs its rows beside the tiles
 // (queries, the wait for the last product, storing: some 2000 cycles) and by 5 us before the first key arrives.
 
 #include "kv_kernels.hpp"
@@ -631,7 +631,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const __gr
                         }
                     }
                     // The maximum comes off before the scale: behind it, top c is rounded, from 2^24 on by more than 16 bits can take up,
-                    // and weights would be infinite.  32 operations more to 64 keys: 4096 rows behind 16384 tokens 1442 -> 1470 us.
+                    // and weights would be infinite.  32 operations more to 64 keys: 4096 rows behind 16384 tokens 1440 -> 1463 us,
+                    // and no less with a branch for the rows that need it.
                     const float off = top == -INFINITY ? 0.f : -top;
                     const uint64_t c2 = two(c, c), off2 = two(off, off), raise2 = two(kRaise<T>, kRaise<T>);
                     uint64_t s0 = 0, s1 = 0;

@@ -175,7 +175,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     row sees the prefix and, with ``causal``, the own tokens up to itself; without, all own tokens of its
     sequence (queries on an encoder's states, for one).  ``max_q`` is the most new tokens any sequence has, or more (default:
     the number of rows).  Give it while generating: where the rows of a key head pass 128, a bound of 1 is up to a
-    quarter faster than the default (200 sequences behind 2048 tokens 192 for 237 us).  ``scale`` defaults to ``head_dim ** -0.5``.  ``lse`` is the
+    quarter faster than the default (200 sequences behind 2048 tokens 198 for 245 us).  ``scale`` defaults to ``head_dim ** -0.5``.  ``lse`` is the
     natural logarithm of the sum of exponentials, float32 [tokens, q_heads].  Rows that see nothing get zeros
     and -inf; rows that belong to no sequence are left as they were (undefined where the result is made here).
     ``workspace``: a uint8 tensor of at least ``prefix_attention_workspace`` bytes, 256-byte aligned; default: taken from torch's
